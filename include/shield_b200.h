@@ -60,7 +60,8 @@ enum {
     SHIELD_TYPE_Q4_1 = 3,
     SHIELD_TYPE_Q5_0 = 6,
     SHIELD_TYPE_Q5_1 = 7,
-    SHIELD_TYPE_Q8_0 = 8
+    SHIELD_TYPE_Q8_0 = 8,
+    SHIELD_TYPE_BF16 = 30 /* caches and their operators only; no weight kernel */
 };
 
 /*
@@ -207,6 +208,133 @@ shield_status shield_seq_length(shield_ctx *ctx, int64_t seq, int32_t *length);
 shield_status shield_seq_reset(shield_ctx *ctx, int64_t seq);
 /* Frees the sequence's device memory. */
 shield_status shield_seq_release(shield_ctx *ctx, int64_t seq);
+
+/*
+ * Paged key/value caches, for batches whose sequences share a prompt: many
+ * requests behind one policy, several questions to one document. Next to the
+ * sequences above, whose caches are contiguous, f32 and exact, a paged cache
+ * holds F16 or BF16, its memory is handed out in pages, sequences forked from
+ * one another share the pages of what they have in common, and the attention
+ * over a batch reads and multiplies a shared run of pages once for all of its
+ * sequences. No counterpart in the reference, whose KvCache is one f32 array
+ * per layer.
+ *
+ * A pool's keys and values are two arrays [n_layers][n_pages][n_kv_heads]
+ * [page_tokens][head_dim]. Position p of a sequence is row p % page_tokens of
+ * page number pages[p / page_tokens]. Pages are counted: a page is free when
+ * no sequence holds it, and the lowest free page is handed out first. Full
+ * pages may be shared; a sequence's last, partly filled page never is, so
+ * adding positions never disturbs another sequence.
+ *
+ * Streams: `stream` is the cudaStream_t on which a call enqueues its GPU work,
+ * null for the context's own stream of that GPU (cudaStreamLegacy names the
+ * default stream). No call here waits for the GPU, except that creating and
+ * releasing may. Bookkeeping happens at the call, so calls on one cache that
+ * use different streams are ordered by the caller (events), a page freed in
+ * one call and handed out in the next among them. Device pointers belong to
+ * the cache's GPU, whichever device is current; the current device is left as
+ * it was.
+ */
+typedef struct shield_kv_config {
+    uint32_t type;       /* SHIELD_TYPE_F16 or SHIELD_TYPE_BF16 */
+    int32_t n_layers, n_kv_heads;
+    int32_t head_dim;    /* 64 or 128 */
+    int32_t page_tokens; /* 16, 32, 64 or 128 */
+    int32_t n_pages;     /* n_pages * page_tokens < 2^31 */
+    void *k, *v;         /* the caller's device memory (128-byte aligned, kept by the caller until
+                            release), or both null: the library allocates */
+} shield_kv_config;
+
+typedef struct shield_kv_info {
+    int32_t n_pages, pages_used;
+    int32_t pages_spanned; /* one past the highest page in use: pages from here on can go back */
+    int32_t n_seqs, page_tokens;
+    void *k, *v;
+} shield_kv_info;
+
+shield_status shield_kv_create(shield_ctx *ctx, int32_t device, const shield_kv_config *cfg, int64_t *kv);
+/* Frees the cache, its sequences and its batches; work that uses them has finished. */
+shield_status shield_kv_release(shield_ctx *ctx, int64_t kv);
+shield_status shield_kv_get_info(shield_ctx *ctx, int64_t kv, shield_kv_info *out);
+
+/* n empty sequences. */
+shield_status shield_kv_open(shield_ctx *ctx, int64_t kv, int32_t n, int64_t *seqs);
+/* Adds counts[i] positions to sequence seqs[i] (each once per call), for
+ * shield_kv_write to fill. SHIELD_ERR_NOMEM when the pool has too few free
+ * pages; nothing is changed then. */
+shield_status shield_kv_extend(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *counts, int32_t n);
+/* n new sequences: out[i] holds the first lens[i] positions (lens null: all)
+ * of seqs[i], which may appear any number of times. Full pages are shared;
+ * the rows of a partly filled last page are copied to a page of out[i]'s own,
+ * all of the call's in one launch (per 300). The pages' other rows keep what
+ * they held. SHIELD_ERR_NOMEM as above. */
+shield_status shield_kv_fork(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *lens, int32_t n,
+                             int64_t *out, void *stream);
+/* As shield_kv_fork, sharing nothing: every row is copied. */
+shield_status shield_kv_copy(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *lens, int32_t n,
+                             int64_t *out, void *stream);
+/* Ends the sequences (each once per call); pages no one else holds are free. */
+shield_status shield_kv_free(shield_ctx *ctx, int64_t kv, const int64_t *seqs, int32_t n);
+/* Packs the pool: the highest used page moves to the lowest free one, and so
+ * on until the used pages are the lowest ones. Sequences keep their contents;
+ * batches have to be set again. moved (optional): pages moved. */
+shield_status shield_kv_compact(shield_ctx *ctx, int64_t kv, int32_t *moved, void *stream);
+/* lengths[i] (optional): positions sequence seqs[i] holds; pages (optional):
+ * its page numbers in pages[i * max_pages ..], padded with -1, SHIELD_ERR_RANGE
+ * when there are more than max_pages. */
+shield_status shield_kv_pages(shield_ctx *ctx, int64_t kv, const int64_t *seqs, int32_t n, int32_t *lengths,
+                              int32_t *pages, int32_t max_pages);
+
+/*
+ * A batch is the plan of one step, used for every layer: which positions are
+ * new, and how the attention's work is cut. Its memory (the plan on the GPU,
+ * partial results) is allocated here for the given capacities and never grows;
+ * it belongs to one step at a time, so steps that may run at the same time use
+ * batches of their own.
+ */
+typedef struct shield_kv_batch_config {
+    int32_t n_heads;       /* query heads, a multiple of n_kv_heads */
+    int32_t max_tokens;    /* new tokens of a step */
+    int32_t max_seqs;
+    int32_t max_positions; /* of the longest sequence */
+} shield_kv_batch_config;
+shield_status shield_kv_batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_config *cfg, int64_t *batch);
+shield_status shield_kv_batch_release(shield_ctx *ctx, int64_t batch);
+/*
+ * Plans a step: the last counts[i] positions of sequence seqs[i] (each once
+ * per call; a count may be 0) are the step's tokens, packed in this order in
+ * the calls below. Runs of pages that several of the sequences share are found
+ * here. The plan holds until one of its sequences is freed or pages move
+ * (SHIELD_ERR_STATE from then on). It cannot be captured into a graph, but
+ * shield_kv_write and shield_kv_attend can: a replay works on the plan set
+ * last before it, of any size within the capacities, and the caller sees to it
+ * that this plan still holds and that the buffers captured are large enough.
+ */
+shield_status shield_kv_batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const int32_t *counts, int32_t n,
+                                  void *stream);
+/*
+ * The step's keys and values of one layer into the pool. k, v: device rows of
+ * n_kv_heads * head_dim values, one per token, k_stride / v_stride elements
+ * apart (0: packed; 16-byte aligned), SHIELD_TYPE_F32 (rounded to nearest) or
+ * the cache's own type.
+ */
+shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t type, const void *k,
+                              int64_t k_stride, const void *v, int64_t v_stride, void *stream);
+/*
+ * The step's causal attention in one layer: for every token and query head,
+ *   out = sum_l w_l v_l / sum_l w_l,   w_l = exp(scale * q . k_l),
+ * over the positions l of its sequence up to and including its own. q, out:
+ * device rows of n_heads * head_dim values of the cache's type, q_stride /
+ * out_stride elements apart (0: packed; 16-byte aligned); query head h reads
+ * kv head h / (n_heads / n_kv_heads). out may be q. Keys and values behind a
+ * token's position have no effect on it, whatever they hold. Scores and sums
+ * are f32, weights are rounded to the cache's type for the product with the
+ * values. The order of the sums, and so the last bits, depend on how the plan
+ * cuts the work: on the batch's lengths and on what is shared; the same plan
+ * gives the same bits.
+ */
+shield_status shield_kv_attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q, int64_t q_stride, void *out,
+                               int64_t out_stride, float scale, void *stream);
 
 /*
  * QuantMatMul.ForwardAsync / ForwardRowsAsync (Numerics/QuantMatMul.cs:71-110)

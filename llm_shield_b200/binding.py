@@ -52,6 +52,25 @@ class ShieldTiming(C.Structure):
                 ("d2h_bytes", C.c_int64), ("attn_ms", C.c_double), ("attn_flops", C.c_double)]
 
 
+class ShieldKvConfig(C.Structure):
+    _fields_ = [("type", C.c_uint32), ("n_layers", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+                ("page_tokens", C.c_int32), ("n_pages", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class ShieldKvInfo(C.Structure):
+    _fields_ = [("n_pages", C.c_int32), ("pages_used", C.c_int32), ("pages_spanned", C.c_int32),
+                ("n_seqs", C.c_int32), ("page_tokens", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class ShieldKvBatchConfig(C.Structure):
+    _fields_ = [("n_heads", C.c_int32), ("max_tokens", C.c_int32), ("max_seqs", C.c_int32),
+                ("max_positions", C.c_int32)]
+
+
+TYPE_F32, TYPE_F16, TYPE_BF16 = 0, 1, 30
+_KV_TYPES = {"f32": TYPE_F32, "f16": TYPE_F16, "bf16": TYPE_BF16}
+
+
 EXPORTS = [
     "shield_open", "shield_close", "shield_device_count", "shield_set_config", "shield_upload_tensor",
     "shield_score_batch", "shield_last_logits", "shield_set_prefix", "shield_get_prefix_state", "shield_prefix_length",
@@ -60,6 +79,9 @@ EXPORTS = [
     "shield_debug_block_dots",
     "shield_set_gemm_path", "shield_set_gemm_tile_width", "shield_set_attention_rows", "shield_debug_activation", "shield_set_timing", "shield_read_timing",
     "shield_device_stream", "shield_last_error",
+    "shield_kv_create", "shield_kv_release", "shield_kv_get_info", "shield_kv_open", "shield_kv_extend",
+    "shield_kv_fork", "shield_kv_copy", "shield_kv_free", "shield_kv_compact", "shield_kv_pages",
+    "shield_kv_batch_create", "shield_kv_batch_release", "shield_kv_batch_set", "shield_kv_write", "shield_kv_attend",
 ]
 
 _lib = None
@@ -102,6 +124,22 @@ def lib() -> C.CDLL:
         L.shield_device_stream.argtypes = [P, C.c_int32, C.POINTER(P)]
         L.shield_set_timing.argtypes = [P, C.c_int32]
         L.shield_read_timing.argtypes = [P, C.c_int32, C.POINTER(ShieldTiming), C.c_int32]
+        I32, I64 = C.c_int32, C.c_int64
+        L.shield_kv_create.argtypes = [P, I32, C.POINTER(ShieldKvConfig), C.POINTER(I64)]
+        L.shield_kv_release.argtypes = [P, I64]
+        L.shield_kv_get_info.argtypes = [P, I64, C.POINTER(ShieldKvInfo)]
+        L.shield_kv_open.argtypes = [P, I64, I32, P]
+        L.shield_kv_extend.argtypes = [P, I64, P, P, I32]
+        L.shield_kv_fork.argtypes = [P, I64, P, P, I32, P, P]
+        L.shield_kv_copy.argtypes = [P, I64, P, P, I32, P, P]
+        L.shield_kv_free.argtypes = [P, I64, P, I32]
+        L.shield_kv_compact.argtypes = [P, I64, C.POINTER(I32), P]
+        L.shield_kv_pages.argtypes = [P, I64, P, I32, P, P, I32]
+        L.shield_kv_batch_create.argtypes = [P, I64, C.POINTER(ShieldKvBatchConfig), C.POINTER(I64)]
+        L.shield_kv_batch_release.argtypes = [P, I64]
+        L.shield_kv_batch_set.argtypes = [P, I64, P, P, I32, P]
+        L.shield_kv_write.argtypes = [P, I64, I32, C.c_uint32, P, I64, P, I64, P]
+        L.shield_kv_attend.argtypes = [P, I64, I32, P, I64, P, I64, C.c_float, P]
         L.shield_last_error.restype = C.c_char_p
         for name in EXPORTS:
             f = getattr(L, name)
@@ -124,6 +162,16 @@ def _check(rc: int):
 
 def _p(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _addr(a: np.ndarray) -> int:
+    return a.__array_interface__["data"][0]
+
+
+def _kv_stream(stream: int | None):
+    """A cudaStream_t for the paged-cache calls: None is the context's own
+    stream, 0 the default stream (cudaStreamLegacy), as torch's handles are."""
+    return None if stream is None else stream or 1
 
 
 def config_from_spec(spec: "synth.ModelSpec", max_positions: int = 0, max_batch_tokens: int = 0) -> ShieldConfig:
@@ -273,6 +321,107 @@ class ShieldContext:
                                         _p(v), n_yes, v.size - n_yes, _p(yes), _p(no), _p(score), _p(logits),
                                         _p(cancel) if cancel is not None else None))
         return yes, no, score, logits
+
+    # Paged caches. Device buffers are addresses (ints), types "f16" / "bf16"
+    # / "f32"; stream: a cudaStream_t, 0 the default stream, None the
+    # context's own stream.
+
+    def kv_create(self, type: str, n_layers: int, n_kv_heads: int, head_dim: int, page_tokens: int, n_pages: int,
+                  k: int | None = None, v: int | None = None, device: int = 0) -> int:
+        """A pool of pages, in the caller's memory (k, v) or the library's."""
+        c = ShieldKvConfig(_KV_TYPES[type], n_layers, n_kv_heads, head_dim, page_tokens, n_pages, k, v)
+        out = C.c_int64()
+        _check(lib().shield_kv_create(self._h, device, C.byref(c), C.byref(out)))
+        return out.value
+
+    def kv_release(self, kv: int) -> None:
+        _check(lib().shield_kv_release(self._h, kv))
+
+    def kv_info(self, kv: int) -> dict:
+        i = ShieldKvInfo()
+        _check(lib().shield_kv_get_info(self._h, kv, C.byref(i)))
+        return {name: getattr(i, name) for name, _ in ShieldKvInfo._fields_}
+
+    def kv_open(self, kv: int, n: int) -> np.ndarray:
+        """n empty sequences."""
+        out = np.empty(max(n, 0), np.int64)
+        _check(lib().shield_kv_open(self._h, kv, n, _addr(out)))
+        return out
+
+    def kv_extend(self, kv: int, seqs, counts) -> None:
+        """Adds counts[i] positions to seqs[i]."""
+        s, c = np.ascontiguousarray(seqs, np.int64), np.ascontiguousarray(counts, np.int32)
+        if s.shape != c.shape or s.ndim != 1:
+            raise ValueError("one count per sequence")
+        _check(lib().shield_kv_extend(self._h, kv, _addr(s), _addr(c), s.size))
+
+    def _kv_children(self, call, kv, seqs, lens, stream):
+        s = np.ascontiguousarray(seqs, np.int64)
+        l = None if lens is None else np.ascontiguousarray(lens, np.int32)
+        if s.ndim != 1 or (l is not None and l.shape != s.shape):
+            raise ValueError("one length per sequence")
+        out = np.empty(s.size, np.int64)
+        _check(call(self._h, kv, _addr(s), None if l is None else _addr(l), s.size, _addr(out), _kv_stream(stream)))
+        return out
+
+    def kv_fork(self, kv: int, seqs, lens=None, stream: int | None = None) -> np.ndarray:
+        """New sequences holding the first lens[i] positions (None: all) of
+        seqs[i], sharing its full pages."""
+        return self._kv_children(lib().shield_kv_fork, kv, seqs, lens, stream)
+
+    def kv_copy(self, kv: int, seqs, lens=None, stream: int | None = None) -> np.ndarray:
+        """As kv_fork, with every row copied."""
+        return self._kv_children(lib().shield_kv_copy, kv, seqs, lens, stream)
+
+    def kv_free(self, kv: int, seqs) -> None:
+        s = np.ascontiguousarray(seqs, np.int64)
+        _check(lib().shield_kv_free(self._h, kv, _addr(s), s.size))
+
+    def kv_compact(self, kv: int, stream: int | None = None) -> int:
+        """Packs the used pages to the pool's start; returns the pages moved."""
+        out = C.c_int32()
+        _check(lib().shield_kv_compact(self._h, kv, C.byref(out), _kv_stream(stream)))
+        return out.value
+
+    def kv_lengths(self, kv: int, seqs) -> np.ndarray:
+        s = np.ascontiguousarray(seqs, np.int64)
+        out = np.empty(s.size, np.int32)
+        _check(lib().shield_kv_pages(self._h, kv, _addr(s), s.size, _addr(out), None, 0))
+        return out
+
+    def kv_pages(self, kv: int, seqs) -> np.ndarray:
+        """The sequences' page numbers, one row each, padded with -1."""
+        s = np.ascontiguousarray(seqs, np.int64)
+        most = -(-int(self.kv_lengths(kv, s).max(initial=0)) // self.kv_info(kv)["page_tokens"])
+        out = np.empty((s.size, most), np.int32)
+        _check(lib().shield_kv_pages(self._h, kv, _addr(s), s.size, None, _addr(out), most))
+        return out
+
+    def kv_batch_create(self, kv: int, n_heads: int, max_tokens: int, max_seqs: int, max_positions: int) -> int:
+        c = ShieldKvBatchConfig(n_heads, max_tokens, max_seqs, max_positions)
+        out = C.c_int64()
+        _check(lib().shield_kv_batch_create(self._h, kv, C.byref(c), C.byref(out)))
+        return out.value
+
+    def kv_batch_release(self, batch: int) -> None:
+        _check(lib().shield_kv_batch_release(self._h, batch))
+
+    def kv_batch_set(self, batch: int, seqs, counts, stream: int | None = None) -> None:
+        """Plans a step on the last counts[i] positions of seqs[i]."""
+        s, c = np.ascontiguousarray(seqs, np.int64), np.ascontiguousarray(counts, np.int32)
+        if s.shape != c.shape or s.ndim != 1:
+            raise ValueError("one count per sequence")
+        _check(lib().shield_kv_batch_set(self._h, batch, _addr(s), _addr(c), s.size, _kv_stream(stream)))
+
+    def kv_write(self, batch: int, layer: int, k: int, v: int, type: str, k_stride: int = 0, v_stride: int = 0,
+                 stream: int | None = None) -> None:
+        """The step's keys and values of one layer into the pool."""
+        _check(lib().shield_kv_write(self._h, batch, layer, _KV_TYPES[type], k, k_stride, v, v_stride, _kv_stream(stream)))
+
+    def kv_attend(self, batch: int, layer: int, q: int, out: int, scale: float, q_stride: int = 0, out_stride: int = 0,
+                  stream: int | None = None) -> None:
+        """The step's causal attention in one layer."""
+        _check(lib().shield_kv_attend(self._h, batch, layer, q, q_stride, out, out_stride, scale, _kv_stream(stream)))
 
     def qmatmul(self, weight: str, x: np.ndarray, M: int, n_out: int, row_ids=None, device: int = 0):
         x = np.ascontiguousarray(x, np.float32)

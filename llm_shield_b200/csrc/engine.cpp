@@ -10,31 +10,21 @@
 #include <memory>
 #include <mutex>
 #include <numeric>
-#include <stdexcept>
 #include <string>
 #include <thread>
 #include <unordered_map>
 #include <vector>
 
+#include "context.h"
+#include "kv.h"
 #include "ops.h"
 #include "shield_b200.h"
 
 namespace shield {
 
-struct Error : std::runtime_error {
-    shield_status code;
-    Error(shield_status c, const std::string &m) : std::runtime_error(m), code(c) {}
-};
-
 static thread_local std::string g_last_error;
 
-#define SHIELD_CUDA(x)                                                                                 \
-    do {                                                                                               \
-        cudaError_t e_ = (x);                                                                          \
-        if (e_ != cudaSuccess)                                                                         \
-            throw Error(e_ == cudaErrorMemoryAllocation ? SHIELD_ERR_NOMEM : SHIELD_ERR_CUDA,          \
-                        std::string(#x) + " failed: " + cudaGetErrorString(e_));                     \
-    } while (0)
+void set_last_error(const char *message) { g_last_error = message; }
 
 static int64_t row_bytes_of(int type, int64_t cols) {
     switch (type) {
@@ -1561,25 +1551,21 @@ using namespace shield;
 
 struct shield_ctx {
     Ctx c;
+    kv::State kv;  // gone before the devices' streams
 };
 
-template <class F>
-static shield_status guarded(F &&f) {
-    try {
-        f();
-        g_last_error.clear();
-        return SHIELD_OK;
-    } catch (const Error &e) {
-        g_last_error = e.what();
-        return e.code;
-    } catch (const std::bad_alloc &) {
-        g_last_error = "host memory exhausted";
-        return SHIELD_ERR_NOMEM;
-    } catch (const std::exception &e) {
-        g_last_error = e.what();
-        return SHIELD_ERR_CUDA;
-    }
+namespace shield {
+
+DeviceView device_view(shield_ctx *ctx, int32_t device) {
+    if (device < 0 || device >= (int32_t)ctx->c.devs.size())
+        throw Error(SHIELD_ERR_RANGE, "device index " + std::to_string(device) + " is outside the context");
+    const Device &d = *ctx->c.devs[device];
+    return {d.ordinal, d.sms, d.stream};
 }
+
+kv::State &kv_state(shield_ctx *ctx) { return ctx->kv; }
+
+}  // namespace shield
 
 extern "C" {
 

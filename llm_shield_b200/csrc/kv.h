@@ -1,0 +1,53 @@
+// Paged key/value caches of a context: the pools, their sequences and the
+// batches whose plans the attention reads.
+#pragma once
+
+#include <memory>
+#include <unordered_map>
+#include <vector>
+
+#include "context.h"
+#include "kv_ops.h"
+
+namespace shield {
+namespace kv {
+
+struct Cache {
+    int64_t id = 0;
+    DeviceView dev;
+    DevPool pool;
+    Pool book;
+    bool owns = false;  // the pool's memory is the library's
+    Cache(const Pool &b) : book(b) {}
+    ~Cache();
+};
+
+struct Batch {
+    Cache *cache = nullptr;
+    int32_t n_heads = 0, max_tokens = 0, max_seqs = 0, max_positions = 0;
+    PlanShape shape;
+    char *dev = nullptr;          // every array of the plan at a fixed offset
+    char *host[2] = {nullptr, nullptr};  // pinned images of it, used in turn
+    cudaEvent_t sent[2] = {nullptr, nullptr};
+    int turn = 0;
+    size_t bytes = 0;
+    float *part_o = nullptr;
+    float2 *part_ml = nullptr;
+    int32_t *err = nullptr;       // error word of the kernels' bounded waits
+    DevPlan plan;
+    Plan last;                    // what was uploaded
+    std::vector<int64_t> seqs;    // the sequences it covers
+    int64_t frees = 0, moves = 0; // the pool's counts when it was planned
+    bool planned = false;
+    ~Batch();
+};
+
+struct State {
+    int64_t next_cache = 1, next_batch = 1;
+    std::unordered_map<int64_t, std::unique_ptr<Cache>> caches;
+    std::unordered_map<int64_t, std::unique_ptr<Batch>> batches;  // destroyed before the caches
+    ~State() { batches.clear(); }
+};
+
+}  // namespace kv
+}  // namespace shield

@@ -1,0 +1,399 @@
+// Attention of a batch of sequences over a paged cache.
+//
+// For a token at position p and query head h of the group of kv head j:
+//   o = sum_{l <= p} w_l v_l / sum w_l,   w_l = 2^(s_l - m),  s_l = scale log2(e) q.k_l
+// with m the running maximum of s. The plan (kv_pool.h) cuts the keys into
+// segments: runs of pages that several sequences share, computed once for the
+// rows of all of them, and the rest of each sequence. A row whose keys lie in
+// several pieces gets a partial (m, sum, unnormalised o) from each, joined by
+// k_attend_merge. Scores, maxima, sums and outputs are f32; the weights are
+// rounded to the cache's type for the product with the values (one rounding of
+// at most half a step, as the output itself has).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+
+#include "kv_ops.h"
+
+namespace shield {
+namespace kv {
+
+// ------------------------------------------------------------ 16-bit types
+
+template <bool BF16>
+struct Half16;
+template <>
+struct Half16<false> {
+    // f16 weights carry a factor 2^14 (it cancels in o / sum): a weight of 2^-38
+    // of the row's largest is still a number, and the largest is far from overflow
+    static constexpr float LIFT = 14.0f;
+    static constexpr uint32_t EXP = 0x7C00u;  // exponent bits: all ones in infinities and NaN
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 r = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+    static __device__ __forceinline__ float value(uint16_t x) { return __half2float(__ushort_as_half(x)); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <>
+struct Half16<true> {
+    static constexpr float LIFT = 0.0f;
+    static constexpr uint32_t EXP = 0x7F80u;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&r);
+    }
+    static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+// Two packed values: whether either is not finite, and the pair with such values as 0.
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint32_t w) {
+    constexpr uint32_t E = Half16<BF16>::EXP;
+    return (w & E) == E || ((w >> 16) & E) == E;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
+    constexpr uint32_t E = Half16<BF16>::EXP;
+    if ((w & E) == E) w &= 0xFFFF0000u;
+    if (((w >> 16) & E) == E) w &= 0x0000FFFFu;
+    return w;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+
+// First element of position `row` of a page: layer, page, kv head.
+__device__ __forceinline__ int64_t row_offset(const DevPool &P, int layer, int page, int head, int row) {
+    return (int64_t)layer * P.layer_stride() +
+           ((((int64_t)page * P.kv_heads + head) << P.page_shift) + row) * P.dim;
+}
+
+// ------------------------------------------------------------- few rows
+
+// Up to 16 rows (a decode step's group of query heads, a short draft) against
+// a run of keys: bound by reading the keys and values once. Four warps take
+// every fourth tile of 16 keys each, with a running (m, sum, o) of their own
+// and their own ring of cp.async stages, so no warp waits for another until
+// the four are joined at the end.
+template <int D>
+struct FewShape {
+    static constexpr int WARPS = 4;
+    static constexpr int KEYS = 16;  // keys of a tile; pages hold a multiple
+    static constexpr int STAGES = D == 128 ? 3 : 4;
+    static constexpr int TILE_BYTES = KEYS * D * 2;
+    static constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // keys, values
+    static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
+    static constexpr int JOIN_BYTES = WARPS * 16 * D * 4;
+    static constexpr int BYTES = RING_BYTES > JOIN_BYTES ? RING_BYTES : JOIN_BYTES;
+};
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
+    using S = FewShape<D>;
+    using H = Half16<BF16>;
+    extern __shared__ __align__(128) uint8_t few_smem[];
+    __shared__ float2 join_ml[S::WARPS][16];
+    __shared__ int dirty;
+    const DevPool &P = A.pool;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t units = (int64_t)A.plan.counts[COUNT_FEW] * P.kv_heads;
+    const uint32_t ring = smem_addr(few_smem) + warp * S::STAGES * S::STAGE_BYTES;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const Item it = A.plan.few[u / P.kv_heads];
+        const int kvh = (int)(u % P.kv_heads);
+        const int32_t *table = A.plan.table + it.table;
+        const int ntiles = (it.k1 - it.k0 + S::KEYS - 1) / S::KEYS;
+        if (threadIdx.x == 0) dirty = 0;
+
+        auto load = [&](int t, int stage) {
+            const int p0 = it.k0 + t * S::KEYS;
+            const int64_t off = row_offset(P, A.layer, table[p0 >> P.page_shift], kvh, p0 & (P.page_tokens - 1));
+            const uint16_t *k = static_cast<const uint16_t *>(P.k) + off, *v = static_cast<const uint16_t *>(P.v) + off;
+            const uint32_t dst = ring + stage * S::STAGE_BYTES;
+#pragma unroll
+            for (int i = 0; i < S::KEYS * D / 8 / 32; i++) {
+                const int idx = i * 32 + lane, row = idx / (D / 8), c = idx % (D / 8);
+                const bool ok = p0 + row < it.k1;
+                const uint32_t to = row * D * 2 + ((c ^ (row & 7)) << 4);
+                copy16(dst + to, ok ? k + idx * 8 : k, ok);
+                copy16(dst + S::TILE_BYTES + to, ok ? v + idx * 8 : v, ok);
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < S::STAGES - 1; s++) {
+            if (warp + s * S::WARPS < ntiles) load(warp + s * S::WARPS, s);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        }
+
+        // this thread's rows: lane / 4 and lane / 4 + 8
+        uint32_t qf[D / 16][4];
+        int lim[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = (lane >> 2) + 8 * e;
+            lim[e] = it.k1;
+            const uint16_t *q = nullptr;
+            if (r < it.nr) {
+                const int at = it.tok0 + (it.r0 + r) / A.group, head = kvh * A.group + (it.r0 + r) % A.group;
+                lim[e] = A.plan.lim[at];
+                q = static_cast<const uint16_t *>(A.q) + A.plan.perm[at] * A.q_stride + head * D + (lane & 3) * 2;
+            }
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                qf[kk][e] = q ? *reinterpret_cast<const uint32_t *>(q + kk * 16) : 0;
+                qf[kk][2 + e] = q ? *reinterpret_cast<const uint32_t *>(q + kk * 16 + 8) : 0;
+            }
+        }
+        const int low = it.masked ? A.plan.lim[it.tok0 + it.r0 / A.group] : it.k1;  // below it every row sees every key
+
+        float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+        float o[D / 8][4];
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        bool found = false;
+
+        int stage = 0;
+        for (int t = warp; t < ntiles; t += S::WARPS) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
+            __syncwarp();
+            const uint32_t ks = ring + stage * S::STAGE_BYTES, vs = ks + S::TILE_BYTES;
+            const int p0 = it.k0 + t * S::KEYS;
+            float c[2][4];
+#pragma unroll
+            for (int j = 0; j < 2; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+            const int mi = lane >> 3, mr = lane & 7;
+#pragma unroll
+            for (int kk = 0; kk < D / 16; kk++) {
+                uint32_t b[4];
+                ldsm4(b, ks + ((mi >> 1) * 8 + mr) * D * 2 + (((2 * kk + (mi & 1)) ^ mr) << 4));
+                H::mma(c[0], qf[kk], b[0], b[1]);
+                H::mma(c[1], qf[kk], b[2], b[3]);
+            }
+            const bool masked = p0 + S::KEYS > low;
+            if (masked) {
+                // values that a row may not see must not reach its product as 0 * inf:
+                // they count as 0 here, and rows that do see them get them at the end
+#pragma unroll
+                for (int i = 0; i < S::KEYS * D / 8 / 32; i++) {
+                    const uint32_t a = vs + (i * 32 + lane) * 16;
+                    uint32_t w[4];
+                    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+                    if (not_finite<BF16>(w[0]) || not_finite<BF16>(w[1]) || not_finite<BF16>(w[2]) || not_finite<BF16>(w[3])) {
+                        found = true;
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(finite_part<BF16>(w[0])),
+                                     "r"(finite_part<BF16>(w[1])), "r"(finite_part<BF16>(w[2])),
+                                     "r"(finite_part<BF16>(w[3])) : "memory");
+                    }
+                }
+                __syncwarp();
+            }
+            uint32_t pf[4];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                float s[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    s[j] = c[j >> 1][2 * e + (j & 1)] * A.scale_log2;
+                    if (masked && p0 + (j >> 1) * 8 + (lane & 3) * 2 + (j & 1) >= lim[e]) s[j] = -INFINITY;
+                }
+                float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                const float mn = fmaxf(m[e], mx);
+                const float ref = mn == -INFINITY ? 0.0f : mn;  // a row with no key so far keeps weights of 0
+                const float old = exp2_approx(m[e] - ref), lift = ref - H::LIFT;
+                m[e] = mn;
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] = exp2_approx(s[j] - lift);
+                sum[e] = __fmaf_rn(sum[e], old, (p[0] + p[1]) + (p[2] + p[3]));
+#pragma unroll
+                for (int i = 0; i < D / 8; i++) {
+                    o[i][2 * e] *= old;
+                    o[i][2 * e + 1] *= old;
+                }
+                pf[e] = H::pack(p[0], p[1]);
+                pf[2 + e] = H::pack(p[2], p[3]);
+            }
+#pragma unroll
+            for (int np = 0; np < D / 16; np++) {
+                uint32_t b[4];
+                ldsm4_trans(b, vs + ((mi & 1) * 8 + mr) * D * 2 + (((2 * np + (mi >> 1)) ^ mr) << 4));
+                H::mma(o[2 * np], pf, b[0], b[1]);
+                H::mma(o[2 * np + 1], pf, b[2], b[3]);
+            }
+            __syncwarp();
+            const int ahead = t + (S::STAGES - 1) * S::WARPS;
+            if (ahead < ntiles) load(ahead, stage == 0 ? S::STAGES - 1 : stage - 1);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            stage = stage + 1 == S::STAGES ? 0 : stage + 1;
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
+            sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+        }
+        __syncthreads();  // every warp is done with its ring; dirty is set to 0
+        float *join = reinterpret_cast<float *>(few_smem);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int r = (lane >> 2) + 8 * e;
+            if ((lane & 3) == 0) join_ml[warp][r] = make_float2(m[e], sum[e]);
+#pragma unroll
+            for (int i = 0; i < D / 8; i++)
+                *reinterpret_cast<float2 *>(join + (warp * 16 + r) * D + i * 8 + (lane & 3) * 2) =
+                    make_float2(o[i][2 * e], o[i][2 * e + 1]);
+        }
+        if (found) dirty = 1;
+        __syncthreads();
+        // 8 threads per row, each D / 8 dims in groups of 4
+        const int r = threadIdx.x >> 3;
+        if (r < it.nr) {
+            float M = -INFINITY, L = 0.0f, w[S::WARPS];
+#pragma unroll
+            for (int i = 0; i < S::WARPS; i++) M = fmaxf(M, join_ml[i][r].x);
+#pragma unroll
+            for (int i = 0; i < S::WARPS; i++) {
+                w[i] = exp2_approx(join_ml[i][r].x - (M == -INFINITY ? 0.0f : M));
+                L = __fmaf_rn(join_ml[i][r].y, w[i], L);
+            }
+            const int at = it.tok0 + (it.r0 + r) / A.group, head = kvh * A.group + (it.r0 + r) % A.group;
+            const int64_t part = it.part + (int64_t)kvh * it.nr + r;
+            const float inv = it.part < 0 ? 1.0f / L : 1.0f;
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) {
+                const int d = j * 32 + (threadIdx.x & 7) * 4;
+                float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int i = 0; i < S::WARPS; i++) {
+                    const float4 x = *reinterpret_cast<const float4 *>(join + (i * 16 + r) * D + d);
+                    a.x = __fmaf_rn(x.x, w[i], a.x);
+                    a.y = __fmaf_rn(x.y, w[i], a.y);
+                    a.z = __fmaf_rn(x.z, w[i], a.z);
+                    a.w = __fmaf_rn(x.w, w[i], a.w);
+                }
+                if (dirty) {
+                    const int end = min(it.k1, A.plan.lim[at]);
+                    for (int p = it.k0 + (max(low - it.k0, 0) / S::KEYS) * S::KEYS; p < end; p++) {
+                        const uint16_t *v = static_cast<const uint16_t *>(P.v) +
+                            row_offset(P, A.layer, table[p >> P.page_shift], kvh, p & (P.page_tokens - 1)) + d;
+                        if ((v[0] & H::EXP) == H::EXP) a.x += H::value(v[0]);
+                        if ((v[1] & H::EXP) == H::EXP) a.y += H::value(v[1]);
+                        if ((v[2] & H::EXP) == H::EXP) a.z += H::value(v[2]);
+                        if ((v[3] & H::EXP) == H::EXP) a.w += H::value(v[3]);
+                    }
+                }
+                if (it.part < 0) {
+                    uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + d;
+                    *reinterpret_cast<uint2 *>(out) = make_uint2(H::pack(a.x * inv, a.y * inv), H::pack(a.z * inv, a.w * inv));
+                } else {
+                    *reinterpret_cast<float4 *>(A.plan.part_o + part * D + d) = a;
+                    if ((threadIdx.x & 7) == 0 && j == 0) A.plan.part_ml[part] = make_float2(M, L);
+                }
+            }
+        }
+        __syncthreads();  // the ring and join_ml are free for the next unit
+    }
+}
+
+template <bool BF16, int D>
+static cudaError_t few_launch(const AttendArgs &A, int64_t units, cudaStream_t s) {
+    using S = FewShape<D>;
+    cudaError_t e = cudaFuncSetAttribute(k_attend_few<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    if (e != cudaSuccess) return e;
+    k_attend_few<BF16, D><<<(unsigned)std::min<int64_t>(units, 1 << 30), 128, S::BYTES, s>>>(A);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s) {
+    if (units == 0) return cudaSuccess;
+    if (A.pool.dim == 128) return A.pool.bf16 ? few_launch<true, 128>(A, units, s) : few_launch<false, 128>(A, units, s);
+    if (A.pool.dim == 64) return A.pool.bf16 ? few_launch<true, 64>(A, units, s) : few_launch<false, 64>(A, units, s);
+    return cudaErrorInvalidValue;
+}
+
+// ----------------------------------------------------------------- joining
+
+// One warp per (token, query head): the row's partials, from its sequence's
+// own keys up through the runs it shares, always in that order.
+template <bool BF16, int D>
+__global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
+    using H = Half16<BF16>;
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    const int heads = A.group * A.pool.kv_heads;
+    const int64_t rows = (int64_t)A.plan.counts[COUNT_MERGE] * heads;
+    for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < rows; w += (int64_t)gridDim.x * 4) {
+        const int at = A.plan.merge[w / heads], head = (int)(w % heads), kvh = head / A.group;
+        float M = -INFINITY, L = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+        for (int sg = A.plan.leaf[at]; sg >= 0;) {
+            const Segment S = A.plan.segs[sg];
+            const int r = (at - S.tok0) * A.group + head % A.group, tile = r / S.tile_rows;
+            for (int sp = 0; sp < S.nsplit; sp++) {
+                const int item = A.plan.where[S.item0 + sp * S.ntiles + tile];
+                if (item < 0) continue;
+                const Item *it = (S.tile_kind ? A.plan.tile : A.plan.few) + item;
+                const int64_t part = it->part + (int64_t)kvh * it->nr + (r - it->r0);
+                const float2 ml = A.plan.part_ml[part];
+                const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
+                const float a = exp2_approx(M - ref), b = exp2_approx(ml.x - ref);
+                M = mn;
+                L = __fmaf_rn(ml.y, b, L * a);
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = __fmaf_rn(A.plan.part_o[part * D + lane * E + e], b, o[e] * a);
+            }
+            sg = S.parent;
+        }
+        const float inv = 1.0f / L;
+        uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = H::pack(o[e] * inv, o[e + 1] * inv);
+    }
+}
+
+template <bool BF16, int D>
+static cudaError_t merge_launch(const AttendArgs &A, int64_t tokens, cudaStream_t s) {
+    const int64_t rows = tokens * A.group * A.pool.kv_heads;
+    k_attend_merge<BF16, D><<<(unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 30), 128, 0, s>>>(A);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attend_merge(const AttendArgs &A, int64_t tokens, cudaStream_t s) {
+    if (tokens == 0) return cudaSuccess;
+    if (A.pool.dim == 128) return A.pool.bf16 ? merge_launch<true, 128>(A, tokens, s) : merge_launch<false, 128>(A, tokens, s);
+    if (A.pool.dim == 64) return A.pool.bf16 ? merge_launch<true, 64>(A, tokens, s) : merge_launch<false, 64>(A, tokens, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kv
+}  // namespace shield
