@@ -43,6 +43,7 @@
 
 #include "common.cuh"
 #include "ops.h"
+#include "ptx.cuh"
 
 namespace shield {
 namespace tc {
@@ -99,100 +100,11 @@ struct Smem {
 
 // ------------------------------------------------------------ PTX helpers
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) {
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-// Bounded wait: gives up after ~2 s of SM clock, raising the CTA's abort flag
-// and the kernel's error word, so a lost arrival can never hang the GPU.
-// Non-blocking test of a phase (the first look of a bounded wait, which on
-// the hot path usually finds the phase complete).
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
-    if (mbar_test(bar, parity)) return true;
-    long long t0 = clock64();
-    for (uint32_t i = 0;; i++) {
-        if (mbar_try(bar, parity)) return true;
-        if ((i & 255) == 255) {
-            if (*abort_flag) return false;
-            if (clock64() - t0 > 4000000000LL) {
-                *abort_flag = 1;
-                if (err) atomicExch(err, 3);
-                return false;
-            }
-        }
-    }
-}
-
-// The same kind of bounded wait for a whole warp: every lane polls and a
-// vote makes the outcome warp-uniform, so a loop around it needs no
-// reconvergence point. It gives up after 2^26 polls (a quarter of a second
-// or more; a preempted CTA does not poll, so time it is not running does not
-// count), raising the abort flag and the error word.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
-    for (uint32_t i = 0;; i++) {
-        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-        if ((i & 255) == 255) {
-            int stop = *abort_flag ? 1 : (i >= (1u << 26) ? 2 : 0);
-            stop = __shfl_sync(0xffffffffu, stop, 0);
-            if (stop) {
-                if (stop == 2 && (threadIdx.x & 31) == 0) {
-                    *abort_flag = 1;
-                    if (err) atomicExch(err, 3);
-                }
-                return false;
-            }
-        }
-    }
-}
-
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
         ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y), "r"(bar)
         : "memory");
-}
-
-__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-// K-major, 128B-swizzled operand: 8-row groups 1024 B apart (SBO), LBO unused (1),
-// descriptor version 1 (sm_100), layout SWIZZLE_128B (2).
-__device__ __forceinline__ uint64_t umma_desc_sw128(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
 // kind::f16 instruction descriptor: D f32, A/B f16, both K-major, M=128, N=TN.
@@ -206,11 +118,6 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64
         "setp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "n"(idesc<TN>()), "r"(accumulate));
-}
-
-__device__ __forceinline__ void umma_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-                 : "memory");
 }
 
 // tcgen05.ld 16x256b.x2: the same for 16 columns (registers 0-7).

@@ -33,7 +33,7 @@ Batch::~Batch() {
     cudaFree(dev);
     cudaFree(part_o);
     cudaFree(part_ml);
-    cudaFree(err);
+    if (err) cudaFreeHost(err);
     if (before >= 0) cudaSetDevice(before);
 }
 
@@ -160,7 +160,6 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     S.group = cfg->n_heads / c.pool.kv_heads;
     S.kv_heads = c.pool.kv_heads;
     S.sms = c.dev.sms;
-    S.few_rows = INT32_MAX;
     S.max_items = 2 * (n + (T * S.group + FEW_TILE - 1) / FEW_TILE) + 4096;
     S.max_segments = 2 * n;
     S.max_part = std::min<int64_t>(262144, 16 * T * cfg->n_heads + 16384);
@@ -185,8 +184,8 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     }
     SHIELD_CUDA(cudaMalloc(&B->part_o, (size_t)S.max_part * c.pool.dim * 4));
     SHIELD_CUDA(cudaMalloc(&B->part_ml, (size_t)S.max_part * sizeof(float2)));
-    SHIELD_CUDA(cudaMalloc(&B->err, 4));
-    SHIELD_CUDA(cudaMemset(B->err, 0, 4));
+    SHIELD_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&B->err), 4, cudaHostAllocMapped));
+    *B->err = 0;
     SHIELD_CUDA(cudaMemset(B->dev, 0, 16));  // no work until a plan is set
     auto ints = [&](size_t o) { return reinterpret_cast<const int32_t *>(B->dev + o); };
     DevPlan &P = B->plan;
@@ -208,9 +207,18 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     st.batches.emplace(*out, std::move(B));
 }
 
+// The kernels' bounded waits report here; the host sees it at the next call.
+static void check_error(Batch &B) {
+    const int32_t e = *static_cast<volatile int32_t *>(B.err);
+    if (!e) return;
+    *B.err = 0;
+    throw Error(SHIELD_ERR_TIMEOUT, "a device-side wait of an earlier call gave up (error word " + std::to_string(e) + ")");
+}
+
 static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const int32_t *counts, int32_t n, void *stream) {
     Batch &B = batch_of(ctx, batch);
     Cache &c = *B.cache;
+    check_error(B);
     need(n, seqs, "seqs");
     need(n, counts, "counts");
     if (n > B.max_seqs)
@@ -270,6 +278,7 @@ static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const
 
 // A plan holds while its sequences live and no page has moved.
 static void check_plan(Batch &B) {
+    check_error(B);
     if (!B.planned) throw Error(SHIELD_ERR_STATE, "the batch has no plan (shield_kv_batch_set)");
     const Pool &book = B.cache->book;
     if (B.moves != book.moves()) throw Error(SHIELD_ERR_STATE, "pages have moved since the batch was set");
@@ -341,7 +350,9 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     // A captured launch replays whatever plan is set then: enough CTAs for any,
     // each striding over the plan's own count.
     const int64_t few = cap ? 2 * (int64_t)c.dev.sms : (int64_t)B.last.few.size() * c.pool.kv_heads;
+    const int64_t tile = cap ? (int64_t)c.dev.sms : (int64_t)B.last.tile.size() * c.pool.kv_heads;
     const int64_t join = cap ? std::min<int64_t>(B.max_tokens, 4096) : (int64_t)B.last.merge.size();
+    check(launch_attend_tile(A, tile, s), "attention, many rows");
     check(launch_attend_few(A, few, s), "attention, few rows");
     check(launch_attend_merge(A, join, s), "attention, joining");
 }

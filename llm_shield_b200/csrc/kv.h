@@ -33,7 +33,7 @@ struct Batch {
     size_t bytes = 0;
     float *part_o = nullptr;
     float2 *part_ml = nullptr;
-    int32_t *err = nullptr;       // error word of the kernels' bounded waits
+    int32_t *err = nullptr;       // error word of the kernels' bounded waits, in mapped host memory
     DevPlan plan;
     Plan last;                    // what was uploaded
     std::vector<int64_t> seqs;    // the sequences it covers

@@ -9,72 +9,14 @@
 // k_attend_merge. Scores, maxima, sums and outputs are f32; the weights are
 // rounded to the cache's type for the product with the values (one rounding of
 // at most half a step, as the output itself has).
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <algorithm>
 
+#include "kv_half16.cuh"
 #include "kv_ops.h"
 
 namespace shield {
 namespace kv {
 
-// ------------------------------------------------------------ 16-bit types
-
-template <bool BF16>
-struct Half16;
-template <>
-struct Half16<false> {
-    // f16 weights carry a factor 2^14 (it cancels in o / sum): a weight of 2^-38
-    // of the row's largest is still a number, and the largest is far from overflow
-    static constexpr float LIFT = 14.0f;
-    static constexpr uint32_t EXP = 0x7C00u;  // exponent bits: all ones in infinities and NaN
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        const __half2 r = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ float value(uint16_t x) { return __half2float(__ushort_as_half(x)); }
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <>
-struct Half16<true> {
-    static constexpr float LIFT = 0.0f;
-    static constexpr uint32_t EXP = 0x7F80u;
-    static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        const __nv_bfloat162 r = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&r);
-    }
-    static __device__ __forceinline__ float value(uint16_t x) { return __uint_as_float((uint32_t)x << 16); }
-    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-
-// Two packed values: whether either is not finite, and the pair with such values as 0.
-template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    constexpr uint32_t E = Half16<BF16>::EXP;
-    return (w & E) == E || ((w >> 16) & E) == E;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t finite_part(uint32_t w) {
-    constexpr uint32_t E = Half16<BF16>::EXP;
-    if ((w & E) == E) w &= 0xFFFF0000u;
-    if (((w >> 16) & E) == E) w &= 0x0000FFFFu;
-    return w;
-}
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -86,12 +28,6 @@ __device__ __forceinline__ void ldsm4_trans(uint32_t (&r)[4], uint32_t a) {
 }
 __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-
-// First element of position `row` of a page: layer, page, kv head.
-__device__ __forceinline__ int64_t row_offset(const DevPool &P, int layer, int page, int head, int row) {
-    return (int64_t)layer * P.layer_stride() +
-           ((((int64_t)page * P.kv_heads + head) << P.page_shift) + row) * P.dim;
 }
 
 // ------------------------------------------------------------- few rows

@@ -1,0 +1,597 @@
+// Attention of many rows over a paged cache, on the 5th-generation tensor
+// cores: prompts, and runs of keys that a whole batch shares.
+//
+// A work unit is an item of the plan (up to 256 rows: tokens times the query
+// heads of one kv head) and its run of keys, taken in blocks of 128. Per row
+// tile of 128 rows and key block:
+//   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
+//   P = 2^(scale S - m), rounded to the cache's type, over S's own TMEM columns
+//   O += P V    tcgen05.mma with P read from TMEM, O (f32) in TMEM
+// The products of one tile run while the other tile's exponentials are taken,
+// so the tensor pipe and the exponential unit (as scarce: 16 per SM and cycle,
+// which is 1024 cycles for the 128 x 128 weights that two products of 512
+// cycles each use) both stay busy. Up to 128 rows there is one row tile and
+// the two take alternate key blocks, each with its own (m, sum, O), joined at
+// the end.
+//
+//   warps 0-3, 4-7  one softmax warpgroup per tile, a thread per row: loads its
+//                   queries, turns S into P, rescales O when the row's maximum
+//                   has grown by more than 2^8 (until then the old one serves:
+//                   weights stay below 2^8 and the factor cancels in O / sum),
+//                   writes the output or the partial result
+//   warp 8          TMA: key and value blocks, page by page, into one ring
+//   warp 9          owns TMEM, issues the products (10 and 11 only complete the
+//                   warpgroup, which hands its registers over as one)
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+#include "kv_half16.cuh"
+#include "kv_ops.h"
+#include "ptx.cuh"
+
+namespace shield {
+namespace kv {
+
+using namespace tc;
+
+// Three warpgroups. At launch every thread has 168 registers (64,512 in all);
+// the two softmax warpgroups then take 224 each, a row of S needing 128, and
+// the third keeps 56: 256 * 224 + 128 * 56 = 64,512.
+constexpr int TILE_THREADS = 384;
+constexpr int ROWS = 128;      // rows of a tile
+constexpr int BLOCK = 128;     // keys of a block
+constexpr float GROWTH = 8.0f; // log2 of how far a maximum may grow before O is rescaled
+
+template <int D>
+struct TileShape {
+    static constexpr int HALVES = D / 64;             // 128-byte wide operand panels
+    static constexpr int PANEL = 128 * 128;           // bytes of 128 rows of one panel
+    static constexpr int SLOT = HALVES * PANEL;       // a key or value block, or a row tile's queries
+    static constexpr int STAGES = D == 128 ? 5 : 8;
+    static constexpr int OFF_RING = 2 * SLOT;
+    static constexpr int OFF_BAR = OFF_RING + STAGES * SLOT;
+    static constexpr int OFF_MISC = OFF_BAR + (8 + 2 * STAGES) * 8;
+    static constexpr int OFF_JOIN = OFF_MISC + 16;    // (m, sum) of the second tile's rows
+    static constexpr int BYTES = OFF_JOIN + ROWS * 8 + 1024;
+    static_assert(ROWS * D * 4 == 2 * SLOT, "one tile's f32 outputs take the queries' place");
+    static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
+};
+
+struct TileArgs {
+    AttendArgs a;
+    CUtensorMap k, v;  // [layer * pages][kv head][row][dim], boxes of a page's rows by 64 dims
+};
+
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap *map, int x, int head, int page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(0), "r"(head), "r"(page), "r"(bar)
+        : "memory");
+}
+
+// MN-major operand (the values: dims contiguous), 128B-swizzled: panels of 64
+// dims LBO apart, groups of 8 keys 1024 bytes (SBO) apart.
+__device__ __forceinline__ uint64_t umma_desc_values(uint32_t saddr, uint32_t panel) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Instruction descriptors: f32 result, 16-bit operands, M = 128.
+template <bool BF16>
+constexpr uint32_t idesc_scores() {
+    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(BLOCK >> 3) << 17) | (8u << 24);
+}
+template <bool BF16, int D>
+constexpr uint32_t idesc_values() {  // the second operand is MN-major
+    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+}
+
+template <uint32_t IDESC>
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "n"(IDESC), "r"(accumulate) : "memory");
+}
+template <uint32_t IDESC>
+__device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "n"(IDESC), "r"(accumulate) : "memory");
+}
+
+#define R8(r, i) "=r"((r)[i]), "=r"((r)[i + 1]), "=r"((r)[i + 2]), "=r"((r)[i + 3]), "=r"((r)[i + 4]), "=r"((r)[i + 5]), "=r"((r)[i + 6]), "=r"((r)[i + 7])
+#define W8(r, i) "r"((r)[i]), "r"((r)[i + 1]), "r"((r)[i + 2]), "r"((r)[i + 3]), "r"((r)[i + 4]), "r"((r)[i + 5]), "r"((r)[i + 6]), "r"((r)[i + 7])
+
+// 32 columns of this warp's 32 TMEM lanes, a lane per thread.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_load32_wait(uint32_t addr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : R8(r, 0), R8(r, 8), R8(r, 16), R8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::W8(r, 0), W8(r, 8), W8(r, 16), W8(r, 24), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// All 128 columns of a row of S, defined after the wait.
+__device__ __forceinline__ void tmem_load128_wait(uint32_t addr, uint32_t (&r)[128]) {
+    tmem_load32(addr, r);
+    tmem_load32(addr + 32, r + 32);
+    tmem_load32(addr + 64, r + 64);
+    tmem_load32(addr + 96, r + 96);
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 128; i++) asm volatile("" : "+r"(r[i]));  // no use may move above the wait
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// One work unit as every role sees it.
+struct Unit {
+    Item it;
+    int kvh, nb;     // kv head, key blocks
+    bool wide;       // two row tiles
+    int lead, ahead; // key blocks whose scores run ahead of their weights, and how many there are
+    int clean;       // whole key blocks that no row is masked in
+    uint32_t ring;   // ring slots filled by earlier units
+    __device__ __forceinline__ Unit(const AttendArgs &A, int64_t u, uint32_t ring_) : ring(ring_) {
+        it = A.plan.tile[u / A.pool.kv_heads];
+        kvh = (int)(u % A.pool.kv_heads);
+        nb = (it.k1 - it.k0 + BLOCK - 1) / BLOCK;
+        wide = it.nr > ROWS;
+        lead = wide ? 1 : 2;
+        ahead = min(lead, nb);
+        const int low = it.masked ? A.plan.lim[it.tok0 + it.r0 / A.group] : it.k1;  // below it every row sees every key
+        clean = max(low - it.k0, 0) / BLOCK;
+    }
+    // The ring's order: the first `ahead` key blocks, then value block i
+    // followed by key block i + lead while there is one.
+    __device__ __forceinline__ uint32_t key_slot(int b) const { return ring + (b < ahead ? b : ahead + 2 * (b - lead) + 1); }
+    __device__ __forceinline__ uint32_t value_slot(int b) const { return ring + ahead + b + min(b, nb - ahead); }
+    __device__ __forceinline__ int blocks_of(int tile) const { return wide ? nb : (nb - tile + 1) / 2; }
+};
+
+template <bool BF16, int D>
+__global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_constant__ TileArgs args) {
+    using S = TileShape<D>;
+    using H = Half16<BF16>;
+    // f16 weights carry a factor 2^LIFT here (with the growth, at most 2^14 in all)
+    constexpr float LIFT = H::LIFT > GROWTH ? H::LIFT - GROWTH : 0.0f;
+    const AttendArgs &A = args.a;
+    const DevPool &P = A.pool;
+    extern __shared__ uint8_t tile_smem[];
+    const uint32_t base = (smem_u32(tile_smem) + 1023) & ~1023u;
+    uint8_t *const smem = tile_smem + (base - smem_u32(tile_smem));
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    const uint32_t bars = base + S::OFF_BAR;
+    auto q_full = [&](int a) { return bars + 8 * a; };
+    auto s_full = [&](int a) { return bars + 16 + 8 * a; };
+    auto p_full = [&](int a) { return bars + 32 + 8 * a; };
+    auto o_full = [&](int a) { return bars + 48 + 8 * a; };
+    auto full = [&](int s) { return bars + 64 + 8 * s; };
+    auto empty = [&](int s) { return bars + 64 + 8 * (S::STAGES + s); };
+    uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_MISC);
+    volatile int *const stop = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 4);
+    volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);  // [2], by the unit's parity
+    float2 *const join_ml = reinterpret_cast<float2 *>(smem + S::OFF_JOIN);
+
+    if (threadIdx.x == 0) {
+        for (int a = 0; a < 2; a++) {
+            mbar_init(q_full(a), ROWS);
+            mbar_init(s_full(a), 1);
+            mbar_init(p_full(a), 4);
+            mbar_init(o_full(a), 1);
+        }
+        for (int s = 0; s < S::STAGES; s++) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        *stop = dirty[0] = dirty[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;  // S and P of tile a at 128 a, O at 256 + 128 a
+
+    const int64_t units = (int64_t)A.plan.counts[COUNT_TILE] * P.kv_heads;
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // ------------------------------------------------- TMA producer
+            const int per = BLOCK >> P.page_shift;  // pages of a block
+            uint32_t ring = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
+                const Unit U(A, u, ring);
+                const int32_t *const table = A.plan.table + U.it.table;
+                auto fill = [&](uint32_t slot, int b, const CUtensorMap *map) {
+                    const int s = slot % S::STAGES;
+                    if (!mbar_wait_warp(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
+                    const int p0 = U.it.k0 + b * BLOCK;
+                    const int pages = min(per, (U.it.k1 - p0 + P.page_tokens - 1) >> P.page_shift);
+                    if (lane == 0) mbar_expect_tx(full(s), (uint32_t)pages * P.page_tokens * D * 2);
+                    __syncwarp();
+                    const int page = lane / S::HALVES, half = lane % S::HALVES;
+                    if (page < pages)
+                        tma_load_page(base + S::OFF_RING + s * S::SLOT + half * S::PANEL + page * P.page_tokens * 128, map, half * 64,
+                                      U.kvh, A.layer * P.pages + table[(p0 >> P.page_shift) + page], full(s));
+                    return true;
+                };
+                for (int b = 0; ok && b < U.ahead; b++) ok = fill(U.key_slot(b), b, &args.k);
+                for (int b = 0; ok && b < U.nb; b++) {
+                    ok = fill(U.value_slot(b), b, &args.v);
+                    if (ok && b + U.lead < U.nb) ok = fill(U.key_slot(b + U.lead), b + U.lead, &args.k);
+                }
+                ring += 2 * U.nb;
+            }
+        } else if (warp == 9 && lane == 0) {
+            // ----------------------------------------------------- products
+            uint32_t ring = 0, turn = 0, done0 = 0, done1 = 0;  // done: key blocks of each tile in earlier units
+            bool ok = true;
+            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x, turn++) {
+                const Unit U(A, u, ring);
+                auto scores = [&](int a, int b) {
+                    const uint32_t slot = U.key_slot(b), s = slot % S::STAGES;
+                    if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    tc_fence_after();
+                    const uint64_t qd = umma_desc_sw128(base + (U.wide ? a * S::SLOT : 0));
+                    const uint64_t kd = umma_desc_sw128(base + S::OFF_RING + s * S::SLOT);
+#pragma unroll
+                    for (int i = 0; i < D / 16; i++) {
+                        const uint32_t off = ((i / 4) * S::PANEL + (i % 4) * 32) >> 4;
+                        mma_smem<idesc_scores<BF16>()>(tmem + 128 * a, qd + off, kd + off, i > 0);
+                    }
+                    if (!U.wide || a == 1) umma_commit(empty(s));
+                    umma_commit(s_full(a));
+                    return true;
+                };
+                auto values = [&](int a, int b, int n) {  // the n-th block of tile a in this unit
+                    if (!mbar_wait(p_full(a), ((a ? done1 : done0) + n) & 1, stop, A.err)) return false;
+                    const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
+                    if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    tc_fence_after();
+                    const uint64_t vd = umma_desc_values(base + S::OFF_RING + s * S::SLOT, S::PANEL);
+#pragma unroll
+                    for (int i = 0; i < BLOCK / 16; i++)
+                        mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
+                    if (!U.wide || a == 1) umma_commit(empty(s));
+                    if (b + U.lead >= U.nb) umma_commit(o_full(a));
+                    return true;
+                };
+                ok = mbar_wait(q_full(0), turn & 1, stop, A.err) && mbar_wait(q_full(1), turn & 1, stop, A.err);
+                if (U.wide) {
+                    ok = ok && scores(0, 0) && scores(1, 0);
+                    for (int b = 0; ok && b < U.nb; b++)
+                        for (int a = 0; ok && a < 2; a++) {
+                            ok = values(a, b, b);
+                            if (ok && b + 1 < U.nb) ok = scores(a, b + 1);
+                        }
+                } else {
+                    for (int b = 0; ok && b < U.ahead; b++) ok = scores(b, b);
+                    for (int b = 0; ok && b < U.nb; b++) {
+                        ok = values(b & 1, b, b >> 1);
+                        if (ok && b + 2 < U.nb) ok = scores(b & 1, b + 2);
+                    }
+                }
+                ring += 2 * U.nb;
+                done0 += U.blocks_of(0);
+                done1 += U.blocks_of(1);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int a = warp >> 2, row = threadIdx.x & 127, group = A.group;
+        const float scale = fmaxf(fabsf(A.scale_log2), 1e-30f);  // a zero scale still keeps masked scores at -inf
+        const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t st = tmem + lanes + 128 * a, ot = tmem + lanes + 256 + 128 * a;
+        uint32_t ring = 0, turn = 0;
+        uint32_t done = 0;          // key blocks of this tile in earlier units
+        uint32_t ends0 = 0, ends1 = 0;  // earlier units in which each tile had a block
+        for (int64_t u = blockIdx.x; u < units; u += gridDim.x, turn++) {
+            const Unit U(A, u, ring);
+            const Item &it = U.it;
+            const int r0 = it.r0 + (U.wide ? a * ROWS : 0), nr = min(ROWS, it.nr - (U.wide ? a * ROWS : 0));
+            if (threadIdx.x == 0) dirty[(turn + 1) & 1] = 0;
+            // queries: 16-byte vectors of rows (one tile each, or half of one) in the
+            // K-major swizzled layout; rows behind the last are 0. A negative scale is
+            // moved into them.
+            {
+                constexpr int VEC = D / 8;
+                const int first = U.wide ? 0 : a * (ROWS / 2);
+                const uint32_t dst = base + (U.wide ? a * S::SLOT : 0);
+#pragma unroll 4
+                for (int i = row; i < (U.wide ? ROWS : ROWS / 2) * VEC; i += 128) {
+                    const int r = first + i / VEC, c = i % VEC;
+                    uint4 x = make_uint4(0, 0, 0, 0);
+                    if (r < nr) {
+                        const int rr = r0 + r, at = it.tok0 + rr / group, head = U.kvh * group + rr % group;
+                        x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(A.q) + A.plan.perm[at] * A.q_stride + head * D + c * 8);
+                        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
+                    }
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * S::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                                 "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                }
+                fence_proxy_async();
+                mbar_arrive(q_full(a));
+            }
+            const bool live = (warp & 3) * 32 < nr;  // some row of this warp exists
+            const int at = it.tok0 + min(r0 + row, r0 + nr - 1) / group;
+            const int lim = row < nr ? min(it.k1, A.plan.lim[at]) : it.k1;
+            float m = -INFINITY, sum = 0.0f;  // m: what the weights are relative to, in log2
+            const int nblocks = U.blocks_of(a);
+            bool ok = true;
+            for (int n = 0; n < nblocks; n++) {
+                const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
+                if (b >= U.clean && (!U.wide || a == 0)) {
+                    // Values that some row may not see must not reach its product as
+                    // 0 * inf, nor may what lies behind the last key: both count as 0
+                    // here, and rows that do see such a value get it at the end.
+                    const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
+                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
+                        ok = false;
+                        break;
+                    }
+                    bool found = false;
+#pragma unroll 4
+                    for (int i = row; i < S::SLOT / 16; i += 128) {
+                        const uint32_t adr = base + S::OFF_RING + s * S::SLOT + i * 16;
+                        const bool inside = p0 + ((i * 16) % S::PANEL) / 128 < it.k1;
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(adr) : "memory");
+                        const bool bad = not_finite<BF16>(w[0]) || not_finite<BF16>(w[1]) || not_finite<BF16>(w[2]) || not_finite<BF16>(w[3]);
+                        found |= bad && inside;
+                        if (bad || !inside)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(adr), "r"(inside ? finite_part<BF16>(w[0]) : 0u),
+                                         "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
+                                         "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
+                    }
+                    if (found) dirty[turn & 1] = 1;
+                    fence_proxy_async();
+                }
+                if (!mbar_wait_warp(s_full(a), (done + n) & 1, stop, A.err)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                if (live) {
+                    uint32_t s[128];
+                    tmem_load128_wait(st, s);
+                    if (b >= U.clean) {
+                        const int seen = lim - p0;
+#pragma unroll
+                        for (int i = 0; i < 128; i++)
+                            if (i >= seen) s[i] = 0xFF800000u;
+                    }
+                    float mx[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) mx[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+                    for (int i = 8; i < 128; i += 2) mx[(i / 2) & 3] = max3(mx[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                    const bool grown = top > m + GROWTH;  // also the first maximum: m is -inf before it
+                    if (__any_sync(0xffffffffu, grown)) {
+                        const float f = grown ? exp2_approx(m - top) : 1.0f;
+                        if (grown) m = top;
+                        sum *= f;
+                        if (n > 0) {  // the products up to the previous block are done: this S came after them
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                tmem_load32_wait(ot + c, o);
+#pragma unroll
+                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                tmem_store32(ot + c, o);
+                            }
+                        }
+                    }
+                    const float shift = (m == -INFINITY ? 0.0f : -m) + LIFT;
+                    const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+                    uint64_t sum2[2] = {0, 0};
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        uint32_t w[32];
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const uint64_t x = fma2(pack2u(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), scale2, shift2);
+                            const float e0 = exp2_approx(lo_f(x)), e1 = exp2_approx(hi_f(x));
+                            sum2[i & 1] = add2(sum2[i & 1], pack2(e0, e1));
+                            w[i] = H::pack(e0, e1);
+                        }
+                        tmem_store32(st + 32 * h, w);
+                    }
+                    sum2[0] = add2(sum2[0], sum2[1]);
+                    sum += lo_f(sum2[0]) + hi_f(sum2[0]);
+                    tmem_store_wait();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full(a));
+            }
+            // ---------------------------------------------------- epilogue
+            if (ok && nblocks > 0) ok = mbar_wait_warp(o_full(a), (a ? ends1 : ends0) & 1, stop, A.err);
+            const bool two = !U.wide && U.nb > 1;  // both warpgroups hold part of the same rows
+            if (two) {
+                if (a == 1) {
+                    // no product reads the queries any more once tile 0 is done too:
+                    // their place takes this tile's outputs, [dim][row]
+                    if (ok) ok = mbar_wait_warp(o_full(0), ends0 & 1, stop, A.err);
+                    if (ok && live) {
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            tmem_load32_wait(ot + c, o);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) *reinterpret_cast<uint32_t *>(smem + ((c + i) * ROWS + row) * 4) = o[i];
+                        }
+                    }
+                    join_ml[row] = make_float2(m, sum);
+                }
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+            }
+            if (ok && live && (U.wide || a == 0)) {
+                tc_fence_after();
+                float f0 = 1.0f, f1 = 0.0f, M = m, L = sum;
+                if (two) {
+                    const float2 other = join_ml[row];
+                    M = fmaxf(m, other.x);
+                    const float ref = M == -INFINITY ? 0.0f : M;
+                    f0 = exp2_approx(m - ref);
+                    f1 = exp2_approx(other.x - ref);
+                    L = __fmaf_rn(other.y, f1, sum * f0);
+                }
+                const bool mine = row < nr;
+                const bool fix = dirty[turn & 1] != 0;
+                const int head = U.kvh * group + (r0 + row) % group;
+                const int64_t part = it.part + (int64_t)U.kvh * it.nr + (r0 + row - it.r0);
+                const float inv = it.part < 0 ? 1.0f / L : 1.0f;
+                // partials of the few-row kernel carry 2^H::LIFT: say the same of these
+                if (mine && it.part >= 0) A.plan.part_ml[part] = make_float2(M + (H::LIFT - LIFT), L);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t o[32];
+                    __syncwarp();  // the load is the whole warp's, rows behind the last included
+                    tmem_load32_wait(ot + c, o);
+                    if (!mine) continue;
+                    if (two) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            const float y = *reinterpret_cast<const float *>(smem + ((c + i) * ROWS + row) * 4);
+                            o[i] = __float_as_uint(__fmaf_rn(y, f1, __uint_as_float(o[i]) * f0));
+                        }
+                    }
+                    if (fix) {
+                        const int32_t *const table = A.plan.table + it.table;
+                        for (int p = it.k0 + U.clean * BLOCK; p < lim; p++) {
+                            const uint16_t *v = static_cast<const uint16_t *>(P.v) +
+                                row_offset(P, A.layer, table[p >> P.page_shift], U.kvh, p & (P.page_tokens - 1)) + c;
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if ((v[i] & H::EXP) == H::EXP) o[i] = __float_as_uint(__uint_as_float(o[i]) + H::value(v[i]));
+                        }
+                    }
+                    if (it.part < 0) {
+                        uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++)
+                                w[j] = H::pack(__uint_as_float(o[i + 2 * j]) * inv, __uint_as_float(o[i + 2 * j + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+                        float *out = A.plan.part_o + part * D + c;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4 *>(out + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+            }
+            tc_fence_before();
+            ring += 2 * U.nb;
+            done += nblocks;
+            ends0++;
+            ends1 += U.blocks_of(1) > 0;
+            // both warpgroups are through with the queries' memory; all leave together
+            // when a wait gave up anywhere
+            int over;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                         "barrier.cta.red.or.pred p, 2, 256, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+                         : "=r"(over) : "r"((!ok || *stop) ? 1 : 0) : "memory");
+            if (over) break;
+        }
+    }
+    __syncthreads();
+    // After a wait gave up, copies and products may still be on their way: give
+    // them a bounded time before the memory they use is let go.
+    if (*stop) {
+        const long long t0 = clock64();
+        while (clock64() - t0 < 400000000LL) __nanosleep(1000);
+        __syncthreads();
+    }
+    if (warp == 9) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    }
+}
+
+// ------------------------------------------------------------------ host
+
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+    if (!fn) {
+        cudaDriverEntryPointQueryResult q;
+        void *p = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+    }
+    return fn;
+}
+
+static bool map_pool(CUtensorMap *m, const DevPool &P, void *data) {
+    auto fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t row = (cuuint64_t)P.dim * 2;
+    cuuint64_t dims[4] = {(cuuint64_t)P.dim, (cuuint64_t)P.page_tokens, (cuuint64_t)P.kv_heads, (cuuint64_t)P.layers * P.pages};
+    cuuint64_t strides[3] = {row, row * P.page_tokens, row * P.page_tokens * P.kv_heads};
+    cuuint32_t box[4] = {64, (cuuint32_t)P.page_tokens, 1, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    return fn(m, P.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, data, dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool BF16, int D>
+static cudaError_t tile_launch(const TileArgs &T, int64_t units, cudaStream_t s) {
+    using S = TileShape<D>;
+    cudaError_t e = cudaFuncSetAttribute(k_attend_tile<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    if (e != cudaSuccess) return e;
+    k_attend_tile<BF16, D><<<(unsigned)std::min<int64_t>(units, 1 << 30), TILE_THREADS, S::BYTES, s>>>(T);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, cudaStream_t s) {
+    if (units == 0) return cudaSuccess;
+    TileArgs T;
+    T.a = A;
+    if (!map_pool(&T.k, A.pool, A.pool.k) || !map_pool(&T.v, A.pool, A.pool.v)) return cudaErrorInvalidValue;
+    if (A.pool.dim == 128) return A.pool.bf16 ? tile_launch<true, 128>(T, units, s) : tile_launch<false, 128>(T, units, s);
+    if (A.pool.dim == 64) return A.pool.bf16 ? tile_launch<true, 64>(T, units, s) : tile_launch<false, 64>(T, units, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kv
+}  // namespace shield
