@@ -352,7 +352,7 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     const int64_t few = cap ? 2 * (int64_t)c.dev.sms : (int64_t)B.last.few.size() * c.pool.kv_heads;
     const int64_t tile = cap ? (int64_t)c.dev.sms : (int64_t)B.last.tile.size() * c.pool.kv_heads;
     const int64_t join = cap ? std::min<int64_t>(B.max_tokens, 4096) : (int64_t)B.last.merge.size();
-    check(launch_attend_tile(A, tile, s), "attention, many rows");
+    check(launch_attend_tile(A, tile, c.dev.sms, s), "attention, many rows");
     check(launch_attend_few(A, few, s), "attention, few rows");
     check(launch_attend_merge(A, join, s), "attention, joining");
 }

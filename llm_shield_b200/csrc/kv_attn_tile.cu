@@ -14,14 +14,17 @@
 // the two take alternate key blocks, each with its own (m, sum, O), joined at
 // the end.
 //
-//   warps 0-3, 4-7  one softmax warpgroup per tile, a thread per row: loads its
-//                   queries, turns S into P, rescales O when the row's maximum
-//                   has grown by more than 2^8 (until then the old one serves:
-//                   weights stay below 2^8 and the factor cancels in O / sum),
-//                   writes the output or the partial result
+//   warps 0-3, 4-7  one softmax warpgroup per tile, a thread per row: turns S
+//                   into P, rescales O when the row's maximum has grown by more
+//                   than 2^8 (until then the old one serves: weights stay below
+//                   2^8 and the factor cancels in O / sum), writes the output or
+//                   the partial result
 //   warp 8          TMA: key and value blocks, page by page, into one ring
-//   warp 9          owns TMEM, issues the products (10 and 11 only complete the
-//                   warpgroup, which hands its registers over as one)
+//   warp 9          owns TMEM, issues the products
+//   warps 10, 11    queries of the next unit, once the last scores of this one
+//                   are done with theirs
+// The grid is persistent, and every role runs on into the next unit as soon as
+// what it needs is there.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -53,12 +56,18 @@ struct TileShape {
     static constexpr int STAGES = D == 128 ? 5 : 8;
     static constexpr int OFF_RING = 2 * SLOT;
     static constexpr int OFF_BAR = OFF_RING + STAGES * SLOT;
-    static constexpr int OFF_MISC = OFF_BAR + (8 + 2 * STAGES) * 8;
+    static constexpr int OFF_MISC = OFF_BAR + (12 + 2 * STAGES) * 8;
     static constexpr int OFF_JOIN = OFF_MISC + 16;    // (m, sum) of the second tile's rows
     static constexpr int BYTES = OFF_JOIN + ROWS * 8 + 1024;
     static_assert(ROWS * D * 4 == 2 * SLOT, "one tile's f32 outputs take the queries' place");
     static_assert(BYTES <= 227 * 1024, "shared memory per CTA");
 };
+
+// The i-th unit of this CTA: longest units first, dealt out forwards and
+// backwards in turn so that every CTA gets about the same.
+__device__ __forceinline__ int64_t dealt(int64_t i) {
+    return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
 
 struct TileArgs {
     AttendArgs a;
@@ -80,6 +89,7 @@ __device__ __forceinline__ uint64_t umma_desc_values(uint32_t saddr, uint32_t pa
 }
 
 // Instruction descriptors: f32 result, 16-bit operands, M = 128.
+constexpr uint32_t NEGATE_A = 1u << 13;
 template <bool BF16>
 constexpr uint32_t idesc_scores() {
     return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(BLOCK >> 3) << 17) | (8u << 24);
@@ -89,12 +99,11 @@ constexpr uint32_t idesc_values() {  // the second operand is MN-major
     return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
 }
 
-template <uint32_t IDESC>
-__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t accumulate) {
+__device__ __forceinline__ void mma_smem(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "n"(IDESC), "r"(accumulate) : "memory");
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 template <uint32_t IDESC>
 __device__ __forceinline__ void mma_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t accumulate) {
@@ -171,6 +180,7 @@ struct Unit {
     // followed by key block i + lead while there is one.
     __device__ __forceinline__ uint32_t key_slot(int b) const { return ring + (b < ahead ? b : ahead + 2 * (b - lead) + 1); }
     __device__ __forceinline__ uint32_t value_slot(int b) const { return ring + ahead + b + min(b, nb - ahead); }
+    __device__ __forceinline__ bool two() const { return !wide && nb > 1; }  // both warpgroups hold part of the same rows
     __device__ __forceinline__ int blocks_of(int tile) const { return wide ? nb : (nb - tile + 1) / 2; }
 };
 
@@ -192,17 +202,20 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     auto s_full = [&](int a) { return bars + 16 + 8 * a; };
     auto p_full = [&](int a) { return bars + 32 + 8 * a; };
     auto o_full = [&](int a) { return bars + 48 + 8 * a; };
-    auto full = [&](int s) { return bars + 64 + 8 * s; };
-    auto empty = [&](int s) { return bars + 64 + 8 * (S::STAGES + s); };
+    auto p_half = [&](int a) { return bars + 64 + 8 * a; };  // the first 64 keys' weights
+    const uint32_t q_free = bars + 80;
+    auto full = [&](int s) { return bars + 96 + 8 * s; };
+    auto empty = [&](int s) { return bars + 96 + 8 * (S::STAGES + s); };
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_MISC);
     volatile int *const stop = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 4);
-    volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);  // [2], by the unit's parity
+    volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);
     float2 *const join_ml = reinterpret_cast<float2 *>(smem + S::OFF_JOIN);
 
     if (threadIdx.x == 0) {
         for (int a = 0; a < 2; a++) {
-            mbar_init(q_full(a), ROWS);
+            mbar_init(q_full(a), 32);
             mbar_init(s_full(a), 1);
+            mbar_init(p_half(a), 4);
             mbar_init(p_full(a), 4);
             mbar_init(o_full(a), 1);
         }
@@ -210,7 +223,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             mbar_init(full(s), 1);
             mbar_init(empty(s), 1);
         }
-        *stop = dirty[0] = dirty[1] = 0;
+        mbar_init(q_free, 2);
+        *stop = *dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 9) {
@@ -230,8 +244,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const int per = BLOCK >> P.page_shift;  // pages of a block
             uint32_t ring = 0;
             bool ok = true;
-            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x) {
-                const Unit U(A, u, ring);
+            for (int64_t i = 0; ok && i * gridDim.x < units; i++) {
+                if (dealt(i) >= units) break;
+                const Unit U(A, dealt(i), ring);
                 const int32_t *const table = A.plan.table + U.it.table;
                 auto fill = [&](uint32_t slot, int b, const CUtensorMap *map) {
                     const int s = slot % S::STAGES;
@@ -256,9 +271,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
         } else if (warp == 9 && lane == 0) {
             // ----------------------------------------------------- products
             uint32_t ring = 0, turn = 0, done0 = 0, done1 = 0;  // done: key blocks of each tile in earlier units
+            const uint32_t score_desc = idesc_scores<BF16>() | (A.scale_log2 < 0.0f ? NEGATE_A : 0u);
             bool ok = true;
-            for (int64_t u = blockIdx.x; ok && u < units; u += gridDim.x, turn++) {
-                const Unit U(A, u, ring);
+            for (int64_t i = 0; ok && i * gridDim.x < units; i++, turn++) {
+                if (dealt(i) >= units) break;
+                const Unit U(A, dealt(i), ring);
                 auto scores = [&](int a, int b) {
                     const uint32_t slot = U.key_slot(b), s = slot % S::STAGES;
                     if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
@@ -268,21 +285,32 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
 #pragma unroll
                     for (int i = 0; i < D / 16; i++) {
                         const uint32_t off = ((i / 4) * S::PANEL + (i % 4) * 32) >> 4;
-                        mma_smem<idesc_scores<BF16>()>(tmem + 128 * a, qd + off, kd + off, i > 0);
+                        mma_smem(tmem + 128 * a, qd + off, kd + off, score_desc, i > 0);
                     }
                     if (!U.wide || a == 1) umma_commit(empty(s));
                     umma_commit(s_full(a));
+                    if (b == U.nb - 1 && (!U.wide || a == 1)) {
+                        // the queries' place is free, unless two warpgroups still join
+                        // their outputs there: they arrive for themselves then
+                        umma_commit(q_free);
+                        if (!U.two()) umma_commit(q_free);
+                    }
                     return true;
                 };
                 auto values = [&](int a, int b, int n) {  // the n-th block of tile a in this unit
-                    if (!mbar_wait(p_full(a), ((a ? done1 : done0) + n) & 1, stop, A.err)) return false;
+                    // the products of the first half run while the other half's weights are taken
+                    const uint32_t ph = ((a ? done1 : done0) + n) & 1;
                     const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
                     if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
-                    tc_fence_after();
                     const uint64_t vd = umma_desc_values(base + S::OFF_RING + s * S::SLOT, S::PANEL);
 #pragma unroll
-                    for (int i = 0; i < BLOCK / 16; i++)
-                        mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
+                    for (int h = 0; h < 2; h++) {
+                        if (!mbar_wait(h ? p_full(a) : p_half(a), ph, stop, A.err)) return false;
+                        tc_fence_after();
+#pragma unroll
+                        for (int i = 4 * h; i < 4 * h + 4; i++)
+                            mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
+                    }
                     if (!U.wide || a == 1) umma_commit(empty(s));
                     if (b + U.lead >= U.nb) umma_commit(o_full(a));
                     return true;
@@ -307,57 +335,78 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 done1 += U.blocks_of(1);
             }
         }
+        if (warp >= 10) {
+            // ---------------------------------------------------- queries
+            // A warp takes a tile's rows, or half of a lone tile's, in 16-byte
+            // vectors, to the K-major swizzled layout; rows behind the last are 0.
+            constexpr int VEC = D / 8, PER = 32 / VEC;  // vectors of a row, rows of one copy
+            const int a = warp - 10;
+            uint32_t turn = 0;
+            bool ok = true;
+            for (int64_t i = 0; ok && i * gridDim.x < units; i++, turn++) {
+                if (dealt(i) >= units) break;
+                const Unit U(A, dealt(i), 0);
+                const int n = U.wide ? ROWS : ROWS / 2, first = a * n;  // of the unit's rows
+                int64_t off[4];  // rows first + lane + 32 j
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int rr = U.it.r0 + min(first + lane + 32 * j, U.it.nr - 1);
+                    off[j] = A.plan.perm[U.it.tok0 + rr / A.group] * A.q_stride + (U.kvh * A.group + rr % A.group) * D;
+                }
+                ok = mbar_wait_warp(q_free, (turn & 1) ^ 1, stop, A.err);
+                if (!ok) break;
+                const int c = lane % VEC;
+                const uint32_t dst = base + (U.wide ? a * S::SLOT : first * 128) + (c >> 3) * S::PANEL;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    if (32 * j >= n) break;
+#pragma unroll 8
+                    for (int k = 0; k < 32; k += PER) {
+                        const int r = 32 * j + k + lane / VEC;
+                        const int64_t o = __shfl_sync(0xffffffffu, off[j], k + lane / VEC);
+                        const bool valid = first + r < U.it.nr;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                                     "l"(static_cast<const uint16_t *>(A.q) + o + c * 8), "r"(valid ? 16 : 0) : "memory");
+                    }
+                }
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                fence_proxy_async();
+                mbar_arrive(q_full(a));
+            }
+        }
         __syncwarp();
     } else {
         // ---------------------------------------------------------- softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int a = warp >> 2, row = threadIdx.x & 127, group = A.group;
         const float scale = fmaxf(fabsf(A.scale_log2), 1e-30f);  // a zero scale still keeps masked scores at -inf
-        const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t st = tmem + lanes + 128 * a, ot = tmem + lanes + 256 + 128 * a;
         uint32_t ring = 0, turn = 0;
         uint32_t done = 0;          // key blocks of this tile in earlier units
         uint32_t ends0 = 0, ends1 = 0;  // earlier units in which each tile had a block
-        for (int64_t u = blockIdx.x; u < units; u += gridDim.x, turn++) {
-            const Unit U(A, u, ring);
+        bool ok = true;  // false once a wait gave up: the remaining units' barriers are still met
+        for (int64_t i = 0; i * gridDim.x < units; i++, turn++) {
+            if (dealt(i) >= units) break;
+            const Unit U(A, dealt(i), ring);
             const Item &it = U.it;
             const int r0 = it.r0 + (U.wide ? a * ROWS : 0), nr = min(ROWS, it.nr - (U.wide ? a * ROWS : 0));
-            if (threadIdx.x == 0) dirty[(turn + 1) & 1] = 0;
-            // queries: 16-byte vectors of rows (one tile each, or half of one) in the
-            // K-major swizzled layout; rows behind the last are 0. A negative scale is
-            // moved into them.
-            {
-                constexpr int VEC = D / 8;
-                const int first = U.wide ? 0 : a * (ROWS / 2);
-                const uint32_t dst = base + (U.wide ? a * S::SLOT : 0);
-#pragma unroll 4
-                for (int i = row; i < (U.wide ? ROWS : ROWS / 2) * VEC; i += 128) {
-                    const int r = first + i / VEC, c = i % VEC;
-                    uint4 x = make_uint4(0, 0, 0, 0);
-                    if (r < nr) {
-                        const int rr = r0 + r, at = it.tok0 + rr / group, head = U.kvh * group + rr % group;
-                        x = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(A.q) + A.plan.perm[at] * A.q_stride + head * D + c * 8);
-                        x = make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
-                    }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c >> 3) * S::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                                 "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-                }
-                fence_proxy_async();
-                mbar_arrive(q_full(a));
-            }
             const bool live = (warp & 3) * 32 < nr;  // some row of this warp exists
             const int at = it.tok0 + min(r0 + row, r0 + nr - 1) / group;
             const int lim = row < nr ? min(it.k1, A.plan.lim[at]) : it.k1;
             float m = -INFINITY, sum = 0.0f;  // m: what the weights are relative to, in log2
             const int nblocks = U.blocks_of(a);
-            bool ok = true;
-            for (int n = 0; n < nblocks; n++) {
+            for (int n = 0; ok && n < nblocks; n++) {
                 const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
+                if (!mbar_wait_warp(s_full(a), (done + n) & 1, stop, A.err)) {
+                    ok = false;
+                    break;
+                }
                 if (b >= U.clean && (!U.wide || a == 0)) {
                     // Values that some row may not see must not reach its product as
                     // 0 * inf, nor may what lies behind the last key: both count as 0
-                    // here, and rows that do see such a value get it at the end.
+                    // here, and rows that do see such a value get it at the end. (Once S is
+                    // there the ring has come to this block: its slot's phase is not an older one.)
                     const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
                     if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
                         ok = false;
@@ -377,12 +426,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                                          "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
                                          "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
                     }
-                    if (found) dirty[turn & 1] = 1;
+                    if (found) *dirty = 1;
                     fence_proxy_async();
-                }
-                if (!mbar_wait_warp(s_full(a), (done + n) & 1, stop, A.err)) {
-                    ok = false;
-                    break;
                 }
                 tc_fence_after();
                 if (live) {
@@ -430,10 +475,18 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                             w[i] = H::pack(e0, e1);
                         }
                         tmem_store32(st + 32 * h, w);
+                        if (h == 0) {
+                            tmem_store_wait();
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(p_half(a));
+                        }
                     }
                     sum2[0] = add2(sum2[0], sum2[1]);
                     sum += lo_f(sum2[0]) + hi_f(sum2[0]);
                     tmem_store_wait();
+                } else if (lane == 0) {
+                    mbar_arrive(p_half(a));
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -441,7 +494,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             }
             // ---------------------------------------------------- epilogue
             if (ok && nblocks > 0) ok = mbar_wait_warp(o_full(a), (a ? ends1 : ends0) & 1, stop, A.err);
-            const bool two = !U.wide && U.nb > 1;  // both warpgroups hold part of the same rows
+            const bool two = U.two();
             if (two) {
                 if (a == 1) {
                     // no product reads the queries any more once tile 0 is done too:
@@ -473,13 +526,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     L = __fmaf_rn(other.y, f1, sum * f0);
                 }
                 const bool mine = row < nr;
-                const bool fix = dirty[turn & 1] != 0;
+                const bool fix = *dirty != 0;  // stays set: the look is right for every unit, and only such data pays for it
                 const int head = U.kvh * group + (r0 + row) % group;
                 const int64_t part = it.part + (int64_t)U.kvh * it.nr + (r0 + row - it.r0);
                 const float inv = it.part < 0 ? 1.0f / L : 1.0f;
                 // partials of the few-row kernel carry 2^H::LIFT: say the same of these
                 if (mine && it.part >= 0) A.plan.part_ml[part] = make_float2(M + (H::LIFT - LIFT), L);
-#pragma unroll 1
+#pragma unroll
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
                     __syncwarp();  // the load is the whole warp's, rows behind the last included
@@ -487,36 +540,37 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     if (!mine) continue;
                     if (two) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float y = *reinterpret_cast<const float *>(smem + ((c + i) * ROWS + row) * 4);
-                            o[i] = __float_as_uint(__fmaf_rn(y, f1, __uint_as_float(o[i]) * f0));
+                        for (int j = 0; j < 32; j++) {
+                            const float y = *reinterpret_cast<const float *>(smem + ((c + j) * ROWS + row) * 4);
+                            o[j] = __float_as_uint(__fmaf_rn(y, f1, __uint_as_float(o[j]) * f0));
                         }
                     }
                     if (fix) {
                         const int32_t *const table = A.plan.table + it.table;
+#pragma unroll 1
                         for (int p = it.k0 + U.clean * BLOCK; p < lim; p++) {
                             const uint16_t *v = static_cast<const uint16_t *>(P.v) +
                                 row_offset(P, A.layer, table[p >> P.page_shift], U.kvh, p & (P.page_tokens - 1)) + c;
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if ((v[i] & H::EXP) == H::EXP) o[i] = __float_as_uint(__uint_as_float(o[i]) + H::value(v[i]));
+                            for (int j = 0; j < 32; j++)
+                                if ((v[j] & H::EXP) == H::EXP) o[j] = __float_as_uint(__uint_as_float(o[j]) + H::value(v[j]));
                         }
                     }
                     if (it.part < 0) {
                         uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + c;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
+                        for (int j = 0; j < 32; j += 8) {
                             uint32_t w[4];
 #pragma unroll
-                            for (int j = 0; j < 4; j++)
-                                w[j] = H::pack(__uint_as_float(o[i + 2 * j]) * inv, __uint_as_float(o[i + 2 * j + 1]) * inv);
-                            *reinterpret_cast<uint4 *>(out + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int k = 0; k < 4; k++)
+                                w[k] = H::pack(__uint_as_float(o[j + 2 * k]) * inv, __uint_as_float(o[j + 2 * k + 1]) * inv);
+                            *reinterpret_cast<uint4 *>(out + j) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     } else {
                         float *out = A.plan.part_o + part * D + c;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4 *>(out + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<uint4 *>(out + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
                     }
                 }
             }
@@ -525,13 +579,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             done += nblocks;
             ends0++;
             ends1 += U.blocks_of(1) > 0;
-            // both warpgroups are through with the queries' memory; all leave together
-            // when a wait gave up anywhere
-            int over;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-                         "barrier.cta.red.or.pred p, 2, 256, q;\n\tselp.b32 %0, 1, 0, p;\n\t}"
-                         : "=r"(over) : "r"((!ok || *stop) ? 1 : 0) : "memory");
-            if (over) break;
+            if (two) {  // the joined outputs have been read: their place is free
+                asm volatile("bar.sync 2, 256;" ::: "memory");
+                if (threadIdx.x == 0) mbar_arrive(q_free);
+            }
         }
     }
     __syncthreads();
@@ -575,21 +626,21 @@ static bool map_pool(CUtensorMap *m, const DevPool &P, void *data) {
 }
 
 template <bool BF16, int D>
-static cudaError_t tile_launch(const TileArgs &T, int64_t units, cudaStream_t s) {
+static cudaError_t tile_launch(const TileArgs &T, int64_t units, int sms, cudaStream_t s) {
     using S = TileShape<D>;
     cudaError_t e = cudaFuncSetAttribute(k_attend_tile<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
     if (e != cudaSuccess) return e;
-    k_attend_tile<BF16, D><<<(unsigned)std::min<int64_t>(units, 1 << 30), TILE_THREADS, S::BYTES, s>>>(T);
+    k_attend_tile<BF16, D><<<(unsigned)std::min<int64_t>(units, sms), TILE_THREADS, S::BYTES, s>>>(T);
     return cudaGetLastError();
 }
 
-cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, cudaStream_t s) {
+cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, int sms, cudaStream_t s) {
     if (units == 0) return cudaSuccess;
     TileArgs T;
     T.a = A;
     if (!map_pool(&T.k, A.pool, A.pool.k) || !map_pool(&T.v, A.pool, A.pool.v)) return cudaErrorInvalidValue;
-    if (A.pool.dim == 128) return A.pool.bf16 ? tile_launch<true, 128>(T, units, s) : tile_launch<false, 128>(T, units, s);
-    if (A.pool.dim == 64) return A.pool.bf16 ? tile_launch<true, 64>(T, units, s) : tile_launch<false, 64>(T, units, s);
+    if (A.pool.dim == 128) return A.pool.bf16 ? tile_launch<true, 128>(T, units, sms, s) : tile_launch<false, 128>(T, units, sms, s);
+    if (A.pool.dim == 64) return A.pool.bf16 ? tile_launch<true, 64>(T, units, sms, s) : tile_launch<false, 64>(T, units, sms, s);
     return cudaErrorInvalidValue;
 }
 

@@ -54,7 +54,7 @@ cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t 
 // The three attention kernels over `units` work units (or as many as a later
 // plan may have: each strides over the plan's own count).
 cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s);
-cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, cudaStream_t s);
+cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, int sms, cudaStream_t s);  // one persistent CTA per SM
 cudaError_t launch_attend_merge(const AttendArgs &A, int64_t tokens, cudaStream_t s);
 
 }  // namespace kv

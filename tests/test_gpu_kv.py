@@ -568,3 +568,24 @@ def test_refusals():
     ctx.kv_write(batch, 0, p, p, "f16", stream=c.stream)
     torch.cuda.synchronize()
     assert not q.any()
+
+
+@pytest.mark.parametrize("shape", [SHAPES[0], SHAPES[1], SHAPES[5]], ids=lambda s: "-".join(map(str, s)))
+def test_more_work_than_the_gpu_holds_at_once(shape):
+    """Several units per CTA, short and long, one tile and two, partial and whole: each the same every time, and right."""
+    type, dim, pt, kv_heads, heads = shape
+    rng = random.Random(7)
+    c = Cache(type, 2, kv_heads, dim, pt, pages=-(-120000 // pt))
+    seqs = np.concatenate([tree(c, rng, roots=3, kids=12, lo=1, hi=1500, own_lo=1, own_hi=300),
+                           tree(c, rng, roots=60, kids=1, lo=1, hi=700, own_lo=1, own_hi=90)])
+    lens = c.ctx.kv_lengths(c.kv, seqs)
+    counts = [min(int(n), rng.choice((1, 3, 6, 20, 34, 70, 200))) for n in lens]
+    b = c.batch(seqs, counts, heads)
+    first = check(c, seqs, counts, heads, batch=b)
+    T = sum(counts)
+    q = torch.randn(T, heads, dim, device="cuda").to(c.dtype)
+    outs = torch.empty(20, T, heads, dim, dtype=c.dtype, device="cuda")
+    for o in outs:
+        c.k.add_(0)  # something else in between
+        c.ctx.kv_attend(b, 1, q.data_ptr(), o.data_ptr(), dim ** -0.5, stream=c.stream)
+    assert torch.equal(outs, outs[:1].expand_as(outs)) and first.shape == outs[0].shape
