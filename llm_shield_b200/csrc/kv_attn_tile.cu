@@ -158,6 +158,17 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// A value that is the same in the whole warp, in a form the compiler knows to
+// be: operands of tcgen05.mma then stay in uniform registers.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elected() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // One work unit as every role sees it.
 struct Unit {
     Item it;
@@ -195,7 +206,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     extern __shared__ uint8_t tile_smem[];
     const uint32_t base = (smem_u32(tile_smem) + 1023) & ~1023u;
     uint8_t *const smem = tile_smem + (base - smem_u32(tile_smem));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     const uint32_t bars = base + S::OFF_BAR;
     auto q_full = [&](int a) { return bars + 8 * a; };
@@ -234,7 +245,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;  // S and P of tile a at 128 a, O at 256 + 128 a
+    const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a at 128 a, O at 256 + 128 a
 
     const int64_t units = (int64_t)A.plan.counts[COUNT_TILE] * P.kv_heads;
     if (warp >= 8) {
@@ -268,61 +279,78 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
                 ring += 2 * U.nb;
             }
-        } else if (warp == 9 && lane == 0) {
+        } else if (warp == 9) {
             // ----------------------------------------------------- products
+            // The whole warp walks the schedule, so that everything in it is
+            // warp-uniform, and one lane issues: with a lone thread in here the
+            // descriptors have to be moved to uniform registers for each product,
+            // and issuing 16 of them took longer than the tensor cores need.
             uint32_t ring = 0, turn = 0, done0 = 0, done1 = 0;  // done: key blocks of each tile in earlier units
             const uint32_t score_desc = idesc_scores<BF16>() | (A.scale_log2 < 0.0f ? NEGATE_A : 0u);
+            const uint64_t q_desc = umma_desc_sw128(base), k_desc = umma_desc_sw128(base + S::OFF_RING);
+            const uint64_t v_desc = umma_desc_values(base + S::OFF_RING, S::PANEL);
+            const bool leader = elected();
             bool ok = true;
             for (int64_t i = 0; ok && i * gridDim.x < units; i++, turn++) {
                 if (dealt(i) >= units) break;
-                const Unit U(A, dealt(i), ring);
+                Unit U(A, dealt(i), ring);
+                U.nb = uniform(U.nb);
+                U.wide = uniform(U.wide) != 0;
+                U.lead = U.wide ? 1 : 2;
+                U.ahead = min(U.lead, U.nb);
                 auto scores = [&](int a, int b) {
                     const uint32_t slot = U.key_slot(b), s = slot % S::STAGES;
-                    if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
                     tc_fence_after();
-                    const uint64_t qd = umma_desc_sw128(base + (U.wide ? a * S::SLOT : 0));
-                    const uint64_t kd = umma_desc_sw128(base + S::OFF_RING + s * S::SLOT);
+                    const uint64_t qd = q_desc + (U.wide ? a * (S::SLOT >> 4) : 0), kd = k_desc + s * (S::SLOT >> 4);
+                    if (leader) {
 #pragma unroll
-                    for (int i = 0; i < D / 16; i++) {
-                        const uint32_t off = ((i / 4) * S::PANEL + (i % 4) * 32) >> 4;
-                        mma_smem(tmem + 128 * a, qd + off, kd + off, score_desc, i > 0);
+                        for (int i = 0; i < D / 16; i++) {
+                            const uint32_t off = ((i / 4) * S::PANEL + (i % 4) * 32) >> 4;
+                            mma_smem(tmem + 128 * a, qd + off, kd + off, score_desc, i > 0);
+                        }
+                        if (!U.wide || a == 1) umma_commit(empty(s));
+                        umma_commit(s_full(a));
+                        if (b == U.nb - 1 && (!U.wide || a == 1)) {
+                            // the queries' place is free, unless two warpgroups still join
+                            // their outputs there: they arrive for themselves then
+                            umma_commit(q_free);
+                            if (!U.two()) umma_commit(q_free);
+                        }
                     }
-                    if (!U.wide || a == 1) umma_commit(empty(s));
-                    umma_commit(s_full(a));
-                    if (b == U.nb - 1 && (!U.wide || a == 1)) {
-                        // the queries' place is free, unless two warpgroups still join
-                        // their outputs there: they arrive for themselves then
-                        umma_commit(q_free);
-                        if (!U.two()) umma_commit(q_free);
-                    }
+                    __syncwarp();
                     return true;
                 };
                 auto values = [&](int a, int b, int n) {  // the n-th block of tile a in this unit
                     // the products of the first half run while the other half's weights are taken
                     const uint32_t ph = ((a ? done1 : done0) + n) & 1;
                     const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
-                    if (!mbar_wait(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
-                    const uint64_t vd = umma_desc_values(base + S::OFF_RING + s * S::SLOT, S::PANEL);
+                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    const uint64_t vd = v_desc + s * (S::SLOT >> 4);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (!mbar_wait(h ? p_full(a) : p_half(a), ph, stop, A.err)) return false;
+                        if (!mbar_wait_warp(h ? p_full(a) : p_half(a), ph, stop, A.err)) return false;
                         tc_fence_after();
+                        if (leader) {
 #pragma unroll
-                        for (int i = 4 * h; i < 4 * h + 4; i++)
-                            mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
+                            for (int i = 4 * h; i < 4 * h + 4; i++)
+                                mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
+                        }
+                        __syncwarp();
                     }
-                    if (!U.wide || a == 1) umma_commit(empty(s));
-                    if (b + U.lead >= U.nb) umma_commit(o_full(a));
+                    if (leader) {
+                        if (!U.wide || a == 1) umma_commit(empty(s));
+                        if (b + U.lead >= U.nb) umma_commit(o_full(a));
+                    }
+                    __syncwarp();
                     return true;
                 };
-                ok = mbar_wait(q_full(0), turn & 1, stop, A.err) && mbar_wait(q_full(1), turn & 1, stop, A.err);
+                ok = mbar_wait_warp(q_full(0), turn & 1, stop, A.err) && mbar_wait_warp(q_full(1), turn & 1, stop, A.err);
                 if (U.wide) {
                     ok = ok && scores(0, 0) && scores(1, 0);
-                    for (int b = 0; ok && b < U.nb; b++)
-                        for (int a = 0; ok && a < 2; a++) {
-                            ok = values(a, b, b);
-                            if (ok && b + 1 < U.nb) ok = scores(a, b + 1);
-                        }
+                    for (int b = 0; ok && b < U.nb; b++) {
+                        ok = values(0, b, b) && (b + 1 >= U.nb || scores(0, b + 1)) && values(1, b, b) && (b + 1 >= U.nb || scores(1, b + 1));
+                    }
                 } else {
                     for (int b = 0; ok && b < U.ahead; b++) ok = scores(b, b);
                     for (int b = 0; ok && b < U.nb; b++) {
