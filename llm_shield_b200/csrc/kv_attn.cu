@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                     uint32_t w[4];
                     asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                                  : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
-                    if (not_finite<BF16>(w[0]) || not_finite<BF16>(w[1]) || not_finite<BF16>(w[2]) || not_finite<BF16>(w[3])) {
+                    if (not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3])) {
                         found = true;
                         asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(finite_part<BF16>(w[0])),
                                      "r"(finite_part<BF16>(w[1])), "r"(finite_part<BF16>(w[2])),

@@ -53,9 +53,10 @@ struct TileShape {
     static constexpr int HALVES = D / 64;             // 128-byte wide operand panels
     static constexpr int PANEL = 128 * 128;           // bytes of 128 rows of one panel
     static constexpr int SLOT = HALVES * PANEL;       // a key or value block, or a row tile's queries
-    static constexpr int STAGES = D == 128 ? 5 : 8;
+    static constexpr int STAGES = D == 128 ? 4 : 8;
     static constexpr int OFF_RING = 2 * SLOT;
-    static constexpr int OFF_BAR = OFF_RING + STAGES * SLOT;
+    static constexpr int OFF_OUT = OFF_RING + STAGES * SLOT;  // 4 KB per softmax warp: outputs on their way to rows
+    static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;
     static constexpr int OFF_MISC = OFF_BAR + (12 + 2 * STAGES) * 8;
     static constexpr int OFF_JOIN = OFF_MISC + 16;    // (m, sum) of the second tile's rows
     static constexpr int BYTES = OFF_JOIN + ROWS * 8 + 1024;
@@ -65,8 +66,8 @@ struct TileShape {
 
 // The i-th unit of this CTA: longest units first, dealt out forwards and
 // backwards in turn so that every CTA gets about the same.
-__device__ __forceinline__ int64_t dealt(int64_t i) {
-    return i * gridDim.x + (i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+__device__ __forceinline__ int dealt(int i) {
+    return i * (int)gridDim.x + (int)(i & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
 }
 
 struct TileArgs {
@@ -177,9 +178,9 @@ struct Unit {
     int lead, ahead; // key blocks whose scores run ahead of their weights, and how many there are
     int clean;       // whole key blocks that no row is masked in
     uint32_t ring;   // ring slots filled by earlier units
-    __device__ __forceinline__ Unit(const AttendArgs &A, int64_t u, uint32_t ring_) : ring(ring_) {
+    __device__ __forceinline__ Unit(const AttendArgs &A, int u, uint32_t ring_) : ring(ring_) {
         it = A.plan.tile[u / A.pool.kv_heads];
-        kvh = (int)(u % A.pool.kv_heads);
+        kvh = u % A.pool.kv_heads;
         nb = (it.k1 - it.k0 + BLOCK - 1) / BLOCK;
         wide = it.nr > ROWS;
         lead = wide ? 1 : 2;
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a at 128 a, O at 256 + 128 a
 
-    const int64_t units = (int64_t)A.plan.counts[COUNT_TILE] * P.kv_heads;
+    const int units = A.plan.counts[COUNT_TILE] * P.kv_heads;  // the host keeps it, and one more round, below 2^31
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
@@ -255,25 +256,36 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const int per = BLOCK >> P.page_shift;  // pages of a block
             uint32_t ring = 0;
             bool ok = true;
-            for (int64_t i = 0; ok && i * gridDim.x < units; i++) {
+            for (int i = 0; ok && i * (int)gridDim.x < units; i++) {
                 if (dealt(i) >= units) break;
                 const Unit U(A, dealt(i), ring);
-                const int32_t *const table = A.plan.table + U.it.table;
+                // The page list in registers, a page per lane, 32 pages and the next 32,
+                // so that no copy waits for its page number: `window` is the first
+                // one's place among the unit's pages, at or before value block b's.
+                const int32_t *const table = A.plan.table + U.it.table + (U.it.k0 >> P.page_shift);
+                const int npages = (U.it.k1 - U.it.k0 + P.page_tokens - 1) >> P.page_shift;
+                int window = 0;
+                int here = lane < npages ? table[lane] : 0, next = 32 + lane < npages ? table[32 + lane] : 0;
                 auto fill = [&](uint32_t slot, int b, const CUtensorMap *map) {
                     const int s = slot % S::STAGES;
+                    const int half = lane % S::HALVES, page = lane / S::HALVES, at = b * per + page - window;
+                    const int x = __shfl_sync(0xffffffffu, here, at & 31), y = __shfl_sync(0xffffffffu, next, at & 31);
                     if (!mbar_wait_warp(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
-                    const int p0 = U.it.k0 + b * BLOCK;
-                    const int pages = min(per, (U.it.k1 - p0 + P.page_tokens - 1) >> P.page_shift);
+                    const int pages = min(per, npages - b * per);
                     if (lane == 0) mbar_expect_tx(full(s), (uint32_t)pages * P.page_tokens * D * 2);
                     __syncwarp();
-                    const int page = lane / S::HALVES, half = lane % S::HALVES;
                     if (page < pages)
                         tma_load_page(base + S::OFF_RING + s * S::SLOT + half * S::PANEL + page * P.page_tokens * 128, map, half * 64,
-                                      U.kvh, A.layer * P.pages + table[(p0 >> P.page_shift) + page], full(s));
+                                      U.kvh, A.layer * P.pages + (at < 32 ? x : y), full(s));
                     return true;
                 };
                 for (int b = 0; ok && b < U.ahead; b++) ok = fill(U.key_slot(b), b, &args.k);
                 for (int b = 0; ok && b < U.nb; b++) {
+                    if (b * per - window >= 32) {
+                        window += 32;
+                        here = next;
+                        next = window + 32 + lane < npages ? table[window + 32 + lane] : 0;
+                    }
                     ok = fill(U.value_slot(b), b, &args.v);
                     if (ok && b + U.lead < U.nb) ok = fill(U.key_slot(b + U.lead), b + U.lead, &args.k);
                 }
@@ -291,7 +303,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const uint64_t v_desc = umma_desc_values(base + S::OFF_RING, S::PANEL);
             const bool leader = elected();
             bool ok = true;
-            for (int64_t i = 0; ok && i * gridDim.x < units; i++, turn++) {
+            for (int i = 0; ok && i * (int)gridDim.x < units; i++, turn++) {
                 if (dealt(i) >= units) break;
                 Unit U(A, dealt(i), ring);
                 U.nb = uniform(U.nb);
@@ -371,7 +383,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const int a = warp - 10;
             uint32_t turn = 0;
             bool ok = true;
-            for (int64_t i = 0; ok && i * gridDim.x < units; i++, turn++) {
+            for (int i = 0; ok && i * (int)gridDim.x < units; i++, turn++) {
                 if (dealt(i) >= units) break;
                 const Unit U(A, dealt(i), 0);
                 const int n = U.wide ? ROWS : ROWS / 2, first = a * n;  // of the unit's rows
@@ -414,7 +426,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
         uint32_t done = 0;          // key blocks of this tile in earlier units
         uint32_t ends0 = 0, ends1 = 0;  // earlier units in which each tile had a block
         bool ok = true;  // false once a wait gave up: the remaining units' barriers are still met
-        for (int64_t i = 0; i * gridDim.x < units; i++, turn++) {
+        for (int i = 0; i * (int)gridDim.x < units; i++, turn++) {
             if (dealt(i) >= units) break;
             const Unit U(A, dealt(i), ring);
             const Item &it = U.it;
@@ -422,6 +434,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const bool live = (warp & 3) * 32 < nr;  // some row of this warp exists
             const int at = it.tok0 + min(r0 + row, r0 + nr - 1) / group;
             const int lim = row < nr ? min(it.k1, A.plan.lim[at]) : it.k1;
+            // where this thread's row goes: the first byte of the output's or the partial's row
+            const int rr = r0 + min(row, nr - 1);
+            char *const own_row = it.part >= 0 ? reinterpret_cast<char *>(A.plan.part_o + (it.part + (int64_t)U.kvh * it.nr + (rr - it.r0)) * D)
+                                               : reinterpret_cast<char *>(static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride +
+                                                                          (U.kvh * group + rr % group) * D);
             float m = -INFINITY, sum = 0.0f;  // m: what the weights are relative to, in log2
             const int nblocks = U.blocks_of(a);
             for (int n = 0; ok && n < nblocks; n++) {
@@ -432,29 +449,39 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
                 if (b >= U.clean && (!U.wide || a == 0)) {
                     // Values that some row may not see must not reach its product as
-                    // 0 * inf, nor may what lies behind the last key: both count as 0
-                    // here, and rows that do see such a value get it at the end. (Once S is
+                    // 0 * inf, nor may what the slot holds behind the last key: what is
+                    // not finite counts as 0 here, and rows that do see such a value get it at the end. (Once S is
                     // there the ring has come to this block: its slot's phase is not an older one.)
                     const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
                     if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
                         ok = false;
                         break;
                     }
-                    bool found = false;
-#pragma unroll 4
-                    for (int i = row; i < S::SLOT / 16; i += 128) {
-                        const uint32_t adr = base + S::OFF_RING + s * S::SLOT + i * 16;
-                        const bool inside = p0 + ((i * 16) % S::PANEL) / 128 < it.k1;
+                    const uint32_t values = base + S::OFF_RING + s * S::SLOT;
+                    uint32_t any = 0;
+#pragma unroll
+                    for (int i = 0; i < S::SLOT / 16 / 128; i++) {
                         uint32_t w[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(adr) : "memory");
-                        const bool bad = not_finite<BF16>(w[0]) || not_finite<BF16>(w[1]) || not_finite<BF16>(w[2]) || not_finite<BF16>(w[3]);
-                        found |= bad && inside;
-                        if (bad || !inside)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(adr), "r"(inside ? finite_part<BF16>(w[0]) : 0u),
-                                         "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
-                                         "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                     : "r"(values + (i * 128 + row) * 16) : "memory");
+                        any |= not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3]);
                     }
-                    if (found) *dirty = 1;
+                    if (any) {
+                        bool found = false;
+#pragma unroll 1
+                        for (int i = row; i < S::SLOT / 16; i += 128) {
+                            const bool inside = p0 + ((i * 16) % S::PANEL) / 128 < it.k1;
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + i * 16) : "memory");
+                            const bool bad = (not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3])) != 0;
+                            found |= bad && inside;
+                            if (bad || !inside)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * 16), "r"(inside ? finite_part<BF16>(w[0]) : 0u),
+                                             "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
+                                             "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
+                        }
+                        if (found) *dirty = 1;
+                    }
                     fence_proxy_async();
                 }
                 tc_fence_after();
@@ -555,17 +582,32 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
                 const bool mine = row < nr;
                 const bool fix = *dirty != 0;  // stays set: the look is right for every unit, and only such data pays for it
-                const int head = U.kvh * group + (r0 + row) % group;
-                const int64_t part = it.part + (int64_t)U.kvh * it.nr + (r0 + row - it.r0);
+                const int64_t part = it.part + (int64_t)U.kvh * it.nr + (r0 - it.r0);
                 const float inv = it.part < 0 ? 1.0f / L : 1.0f;
                 // partials of the few-row kernel carry 2^H::LIFT: say the same of these
-                if (mine && it.part >= 0) A.plan.part_ml[part] = make_float2(M + (H::LIFT - LIFT), L);
+                if (mine && it.part >= 0) A.plan.part_ml[part + row] = make_float2(M + (H::LIFT - LIFT), L);
+                // A thread holds a row; rows go out through shared memory (128 bytes of
+                // each at a time, 16-byte chunks xor-ed with the row against bank
+                // conflicts), so that 8 lanes write 128 bytes of one row together
+                // instead of 32 lanes 16 bytes of 32 rows.
+                const uint32_t stage = base + S::OFF_OUT + warp * 4096;
+                auto flush = [&](int byte) {
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int r = (lane >> 3) + 4 * j;
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                     : "r"(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) : "memory");
+                        char *const to = reinterpret_cast<char *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(own_row), r));
+                        if ((warp & 3) * 32 + r < nr) *reinterpret_cast<uint4 *>(to + byte + (lane & 7) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    __syncwarp();
+                };
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
                     uint32_t o[32];
-                    __syncwarp();  // the load is the whole warp's, rows behind the last included
                     tmem_load32_wait(ot + c, o);
-                    if (!mine) continue;
                     if (two) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) {
@@ -573,7 +615,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                             o[j] = __float_as_uint(__fmaf_rn(y, f1, __uint_as_float(o[j]) * f0));
                         }
                     }
-                    if (fix) {
+                    if (fix && mine) {
                         const int32_t *const table = A.plan.table + it.table;
 #pragma unroll 1
                         for (int p = it.k0 + U.clean * BLOCK; p < lim; p++) {
@@ -584,21 +626,23 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                                 if ((v[j] & H::EXP) == H::EXP) o[j] = __float_as_uint(__uint_as_float(o[j]) + H::value(v[j]));
                         }
                     }
-                    if (it.part < 0) {
-                        uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + c;
+                    auto put = [&](int chunk, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+                    };
+                    if (it.part < 0) {  // two column groups of 32 make 128 bytes
 #pragma unroll
                         for (int j = 0; j < 32; j += 8) {
                             uint32_t w[4];
 #pragma unroll
                             for (int k = 0; k < 4; k++)
                                 w[k] = H::pack(__uint_as_float(o[j + 2 * k]) * inv, __uint_as_float(o[j + 2 * k + 1]) * inv);
-                            *reinterpret_cast<uint4 *>(out + j) = make_uint4(w[0], w[1], w[2], w[3]);
+                            put((c & 32) / 8 + j / 8, w[0], w[1], w[2], w[3]);
                         }
+                        if (c & 32) flush((c - 32) * 2);
                     } else {
-                        float *out = A.plan.part_o + part * D + c;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4)
-                            *reinterpret_cast<uint4 *>(out + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int j = 0; j < 32; j += 4) put(j / 4, o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        flush(c * 4);
                     }
                 }
             }

@@ -45,12 +45,14 @@ struct Half16<true> {
     }
 };
 
-// Two packed values: whether either is not finite, and the pair with such values as 0.
+// Two packed values: bits 15 and 31 tell which of them is not finite (adding the
+// exponent's lowest bit carries out of it only where it is all ones).
 template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint32_t w) {
-    constexpr uint32_t E = Half16<BF16>::EXP;
-    return (w & E) == E || ((w >> 16) & E) == E;
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) {
+    constexpr uint32_t E = Half16<BF16>::EXP, E2 = E | E << 16, ONE = (E & (~E + 1)) * 0x10001u;
+    return ((w & E2) + ONE) & 0x80008000u;
 }
+// The pair with such values as 0.
 template <bool BF16>
 __device__ __forceinline__ uint32_t finite_part(uint32_t w) {
     constexpr uint32_t E = Half16<BF16>::EXP;
