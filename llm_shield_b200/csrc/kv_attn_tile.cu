@@ -20,8 +20,8 @@
 //                   2^8 and the factor cancels in O / sum), writes the output or
 //                   the partial result
 //   warp 8          TMA: key and value blocks, page by page, into one ring
-//   warp 9          owns TMEM, issues the products
-//   warps 10, 11    queries of the next unit, once the last scores of this one
+//   warps 9, 10     one per tile: issue its products (9 owns TMEM)
+//   warp 11         queries of the next unit, once the last scores of this one
 //                   are done with theirs
 // The grid is persistent, and every role runs on into the next unit as soon as
 // what it needs is there.
@@ -45,7 +45,8 @@ using namespace tc;
 // the third keeps 56: 256 * 224 + 128 * 56 = 64,512.
 constexpr int TILE_THREADS = 384;
 constexpr int ROWS = 128;      // rows of a tile
-constexpr int BLOCK = 128;     // keys of a block
+constexpr int BLOCK = 128;     // keys of a block, the step of the ring
+constexpr int HALF = 64;       // keys of one score product: a tile's S has room for two
 constexpr float GROWTH = 8.0f; // log2 of how far a maximum may grow before O is rescaled
 
 template <int D>
@@ -57,7 +58,7 @@ struct TileShape {
     static constexpr int OFF_RING = 2 * SLOT;
     static constexpr int OFF_OUT = OFF_RING + STAGES * SLOT;  // 4 KB per softmax warp: outputs on their way to rows
     static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;
-    static constexpr int OFF_MISC = OFF_BAR + (12 + 2 * STAGES) * 8;
+    static constexpr int OFF_MISC = OFF_BAR + (16 + 2 * STAGES) * 8;
     static constexpr int OFF_JOIN = OFF_MISC + 16;    // (m, sum) of the second tile's rows
     static constexpr int BYTES = OFF_JOIN + ROWS * 8 + 1024;
     static_assert(ROWS * D * 4 == 2 * SLOT, "one tile's f32 outputs take the queries' place");
@@ -93,7 +94,7 @@ __device__ __forceinline__ uint64_t umma_desc_values(uint32_t saddr, uint32_t pa
 constexpr uint32_t NEGATE_A = 1u << 13;
 template <bool BF16>
 constexpr uint32_t idesc_scores() {
-    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(BLOCK >> 3) << 17) | (8u << 24);
+    return (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)(HALF >> 3) << 17) | (8u << 24);
 }
 template <bool BF16, int D>
 constexpr uint32_t idesc_values() {  // the second operand is MN-major
@@ -138,15 +139,13 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t *r) {
         ::W8(r, 0), W8(r, 8), W8(r, 16), W8(r, 24), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// All 128 columns of a row of S, defined after the wait.
-__device__ __forceinline__ void tmem_load128_wait(uint32_t addr, uint32_t (&r)[128]) {
+// 64 columns, defined after the wait.
+__device__ __forceinline__ void tmem_load64_wait(uint32_t addr, uint32_t (&r)[64]) {
     tmem_load32(addr, r);
     tmem_load32(addr + 32, r + 32);
-    tmem_load32(addr + 64, r + 64);
-    tmem_load32(addr + 96, r + 96);
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 128; i++) asm volatile("" : "+r"(r[i]));  // no use may move above the wait
+    for (int i = 0; i < 64; i++) asm volatile("" : "+r"(r[i]));  // no use may move above the wait
 }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t d;
@@ -210,14 +209,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
 
     const uint32_t bars = base + S::OFF_BAR;
-    auto q_full = [&](int a) { return bars + 8 * a; };
-    auto s_full = [&](int a) { return bars + 16 + 8 * a; };
-    auto p_full = [&](int a) { return bars + 32 + 8 * a; };
-    auto o_full = [&](int a) { return bars + 48 + 8 * a; };
-    auto p_half = [&](int a) { return bars + 64 + 8 * a; };  // the first 64 keys' weights
-    const uint32_t q_free = bars + 80;
-    auto full = [&](int s) { return bars + 96 + 8 * s; };
-    auto empty = [&](int s) { return bars + 96 + 8 * (S::STAGES + s); };
+    const uint32_t q_full = bars, q_free = bars + 8;
+    auto s_full = [&](int a, int h) { return bars + 16 + 16 * a + 8 * h; };
+    auto p_full = [&](int a, int h) { return bars + 48 + 16 * a + 8 * h; };
+    auto pv_done = [&](int a) { return bars + 80 + 8 * a; };  // one phase per half block
+    auto o_full = [&](int a) { return bars + 96 + 8 * a; };   // one phase per unit
+    const uint32_t v_clean = bars + 112;  // one phase per value block of two tiles that was looked through
+    auto full = [&](int s) { return bars + 128 + 8 * s; };
+    auto empty = [&](int s) { return bars + 128 + 8 * (S::STAGES + s); };
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_MISC);
     volatile int *const stop = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 4);
     volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);
@@ -225,17 +224,20 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
 
     if (threadIdx.x == 0) {
         for (int a = 0; a < 2; a++) {
-            mbar_init(q_full(a), 32);
-            mbar_init(s_full(a), 1);
-            mbar_init(p_half(a), 4);
-            mbar_init(p_full(a), 4);
+            for (int h = 0; h < 2; h++) {
+                mbar_init(s_full(a, h), 1);
+                mbar_init(p_full(a, h), 4);
+            }
+            mbar_init(pv_done(a), 1);
             mbar_init(o_full(a), 1);
         }
         for (int s = 0; s < S::STAGES; s++) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 1);
+            mbar_init(empty(s), 2);  // one per tile, or twice by the tile whose block it is
         }
-        mbar_init(q_free, 2);
+        mbar_init(v_clean, 4);
+        mbar_init(q_full, 32);
+        mbar_init(q_free, 3);
         *stop = *dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -246,7 +248,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a at 128 a, O at 256 + 128 a
+    const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a's half h at 128 a + 64 h, O at 256 + 128 a
 
     const int units = A.plan.counts[COUNT_TILE] * P.kv_heads;  // the host keeps it, and one more round, below 2^31
     if (warp >= 8) {
@@ -291,16 +293,22 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
                 ring += 2 * U.nb;
             }
-        } else if (warp == 9) {
+        } else if (warp < 11) {
             // ----------------------------------------------------- products
             // The whole warp walks the schedule, so that everything in it is
             // warp-uniform, and one lane issues: with a lone thread in here the
             // descriptors have to be moved to uniform registers for each product,
-            // and issuing 16 of them took longer than the tensor cores need.
-            uint32_t ring = 0, turn = 0, done0 = 0, done1 = 0;  // done: key blocks of each tile in earlier units
+            // and issuing 16 of them took longer than the tensor cores need. A wait
+            // costs some 200 cycles even when its phase is complete (the products'
+            // operands keep shared memory busy), so each block is waited for once,
+            // and each tile has a warp of its own.
+            const int a = warp - 9;
+            uint32_t ring = 0, turn = 0, done = 0;  // done: key blocks of this tile in earlier units
+            uint32_t cleaned = 0;                   // phases of v_clean waited for
             const uint32_t score_desc = idesc_scores<BF16>() | (A.scale_log2 < 0.0f ? NEGATE_A : 0u);
             const uint64_t q_desc = umma_desc_sw128(base), k_desc = umma_desc_sw128(base + S::OFF_RING);
             const uint64_t v_desc = umma_desc_values(base + S::OFF_RING, S::PANEL);
+            const uint32_t st = tmem + 128 * a, ot = tmem + 256 + 128 * a;
             const bool leader = elected();
             bool ok = true;
             for (int i = 0; ok && i * (int)gridDim.x < units; i++, turn++) {
@@ -310,108 +318,104 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 U.wide = uniform(U.wide) != 0;
                 U.lead = U.wide ? 1 : 2;
                 U.ahead = min(U.lead, U.nb);
-                auto scores = [&](int a, int b) {
-                    const uint32_t slot = U.key_slot(b), s = slot % S::STAGES;
-                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                U.clean = uniform(U.clean);
+                const int nblocks = U.blocks_of(a), b0 = U.wide ? 0 : a, step = U.wide ? 1 : 2;
+                const uint64_t qd = q_desc + (U.wide ? a * (S::SLOT >> 4) : 0);
+                auto scores = [&](int n, int h) {  // of half h of this tile's n-th block
+                    const uint32_t slot = U.key_slot(b0 + n * step), s = slot % S::STAGES;
+                    if (h == 0 && !mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
                     tc_fence_after();
-                    const uint64_t qd = q_desc + (U.wide ? a * (S::SLOT >> 4) : 0), kd = k_desc + s * (S::SLOT >> 4);
+                    const uint64_t kd = k_desc + s * (S::SLOT >> 4) + h * (HALF * 128 >> 4);
                     if (leader) {
 #pragma unroll
                         for (int i = 0; i < D / 16; i++) {
                             const uint32_t off = ((i / 4) * S::PANEL + (i % 4) * 32) >> 4;
-                            mma_smem(tmem + 128 * a, qd + off, kd + off, score_desc, i > 0);
+                            mma_smem(st + 64 * h, qd + off, kd + off, score_desc, i > 0);
                         }
-                        if (!U.wide || a == 1) umma_commit(empty(s));
-                        umma_commit(s_full(a));
-                        if (b == U.nb - 1 && (!U.wide || a == 1)) {
-                            // the queries' place is free, unless two warpgroups still join
-                            // their outputs there: they arrive for themselves then
-                            umma_commit(q_free);
-                            if (!U.two()) umma_commit(q_free);
+                        umma_commit(s_full(a, h));
+                        if (h == 1) {
+                            umma_commit(empty(s));
+                            if (!U.wide) umma_commit(empty(s));
+                            if (n == nblocks - 1) {
+                                // The queries' place is free when both tiles and, where two
+                                // warpgroups join their outputs there, these have said so.
+                                umma_commit(q_free);
+                                if (U.wide ? a == 1 : !U.two()) umma_commit(q_free);
+                                if (!U.wide && !U.two()) umma_commit(q_free);
+                            }
                         }
                     }
                     __syncwarp();
                     return true;
                 };
-                auto values = [&](int a, int b, int n) {  // the n-th block of tile a in this unit
-                    // the products of the first half run while the other half's weights are taken
-                    const uint32_t ph = ((a ? done1 : done0) + n) & 1;
-                    const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
-                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                auto values = [&](int n, int h) {
+                    const uint32_t slot = U.value_slot(b0 + n * step), s = slot % S::STAGES;
+                    if (h == 0 && !mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
                     const uint64_t vd = v_desc + s * (S::SLOT >> 4);
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        if (!mbar_wait_warp(h ? p_full(a) : p_half(a), ph, stop, A.err)) return false;
-                        tc_fence_after();
-                        if (leader) {
-#pragma unroll
-                            for (int i = 4 * h; i < 4 * h + 4; i++)
-                                mma_tmem<idesc_values<BF16, D>()>(tmem + 256 + 128 * a, tmem + 128 * a + 8 * i, vd + ((i * 2048) >> 4), n > 0 || i > 0);
-                        }
-                        __syncwarp();
-                    }
+                    if (h == 0 && a == 1 && U.wide && n >= U.clean && !mbar_wait_warp(v_clean, cleaned++ & 1, stop, A.err)) return false;
+                    if (!mbar_wait_warp(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
+                    tc_fence_after();
                     if (leader) {
-                        if (!U.wide || a == 1) umma_commit(empty(s));
-                        if (b + U.lead >= U.nb) umma_commit(o_full(a));
+#pragma unroll
+                        for (int i = 0; i < HALF / 16; i++)
+                            mma_tmem<idesc_values<BF16, D>()>(ot, st + 64 * h + 8 * i, vd + (((4 * h + i) * 2048) >> 4), n > 0 || h > 0 || i > 0);
+                        umma_commit(pv_done(a));
+                        if (h == 1) {
+                            umma_commit(empty(s));
+                            if (!U.wide) umma_commit(empty(s));
+                            if (n == nblocks - 1) umma_commit(o_full(a));
+                        }
                     }
                     __syncwarp();
                     return true;
                 };
-                ok = mbar_wait_warp(q_full(0), turn & 1, stop, A.err) && mbar_wait_warp(q_full(1), turn & 1, stop, A.err);
-                if (U.wide) {
-                    ok = ok && scores(0, 0) && scores(1, 0);
-                    for (int b = 0; ok && b < U.nb; b++) {
-                        ok = values(0, b, b) && (b + 1 >= U.nb || scores(0, b + 1)) && values(1, b, b) && (b + 1 >= U.nb || scores(1, b + 1));
-                    }
-                } else {
-                    for (int b = 0; ok && b < U.ahead; b++) ok = scores(b, b);
-                    for (int b = 0; ok && b < U.nb; b++) {
-                        ok = values(b & 1, b, b >> 1);
-                        if (ok && b + 2 < U.nb) ok = scores(b & 1, b + 2);
-                    }
+                ok = mbar_wait_warp(q_full, turn & 1, stop, A.err);
+                if (nblocks > 0) ok = ok && scores(0, 0) && scores(0, 1);
+                // A half's next scores follow its weights' product, whose operand they
+                // overwrite; the other half's are there already, so the softmax finds
+                // scores whenever it comes back.
+                for (int n = 0; ok && n < nblocks; n++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++) ok = ok && values(n, h) && (n + 1 >= nblocks || scores(n + 1, h));
                 }
                 ring += 2 * U.nb;
-                done0 += U.blocks_of(0);
-                done1 += U.blocks_of(1);
+                done += nblocks;
             }
-        }
-        if (warp >= 10) {
+        } else {
             // ---------------------------------------------------- queries
-            // A warp takes a tile's rows, or half of a lone tile's, in 16-byte
-            // vectors, to the K-major swizzled layout; rows behind the last are 0.
+            // 16-byte vectors to the K-major swizzled layout; rows behind the last
+            // are 0.
             constexpr int VEC = D / 8, PER = 32 / VEC;  // vectors of a row, rows of one copy
-            const int a = warp - 10;
             uint32_t turn = 0;
             bool ok = true;
             for (int i = 0; ok && i * (int)gridDim.x < units; i++, turn++) {
                 if (dealt(i) >= units) break;
                 const Unit U(A, dealt(i), 0);
-                const int n = U.wide ? ROWS : ROWS / 2, first = a * n;  // of the unit's rows
-                int64_t off[4];  // rows first + lane + 32 j
+                int64_t off[8];  // rows lane + 32 j
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int rr = U.it.r0 + min(first + lane + 32 * j, U.it.nr - 1);
+                for (int j = 0; j < 8; j++) {
+                    const int rr = U.it.r0 + min(lane + 32 * j, U.it.nr - 1);
                     off[j] = A.plan.perm[U.it.tok0 + rr / A.group] * A.q_stride + (U.kvh * A.group + rr % A.group) * D;
                 }
                 ok = mbar_wait_warp(q_free, (turn & 1) ^ 1, stop, A.err);
                 if (!ok) break;
                 const int c = lane % VEC;
-                const uint32_t dst = base + (U.wide ? a * S::SLOT : first * 128) + (c >> 3) * S::PANEL;
+                const uint32_t dst = base + (c >> 3) * S::PANEL;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (32 * j >= n) break;
+                for (int j = 0; j < 8; j++) {
+                    if (j >= 4 && !U.wide) break;
+                    const uint32_t tile = dst + (j / 4) * S::SLOT;
 #pragma unroll 8
                     for (int k = 0; k < 32; k += PER) {
                         const int r = 32 * j + k + lane / VEC;
                         const int64_t o = __shfl_sync(0xffffffffu, off[j], k + lane / VEC);
-                        const bool valid = first + r < U.it.nr;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + r * 128 + (((c & 7) ^ (r & 7)) << 4)),
-                                     "l"(static_cast<const uint16_t *>(A.q) + o + c * 8), "r"(valid ? 16 : 0) : "memory");
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tile + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4)),
+                                     "l"(static_cast<const uint16_t *>(A.q) + o + c * 8), "r"(r < U.it.nr ? 16 : 0) : "memory");
                     }
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
                 fence_proxy_async();
-                mbar_arrive(q_full(a));
+                mbar_arrive(q_full);
             }
         }
         __syncwarp();
@@ -443,109 +447,111 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const int nblocks = U.blocks_of(a);
             for (int n = 0; ok && n < nblocks; n++) {
                 const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
-                if (!mbar_wait_warp(s_full(a), (done + n) & 1, stop, A.err)) {
-                    ok = false;
-                    break;
-                }
-                if (b >= U.clean && (!U.wide || a == 0)) {
-                    // Values that some row may not see must not reach its product as
-                    // 0 * inf, nor may what the slot holds behind the last key: what is
-                    // not finite counts as 0 here, and rows that do see such a value get it at the end. (Once S is
-                    // there the ring has come to this block: its slot's phase is not an older one.)
-                    const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
-                    if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
+#pragma unroll 1
+                for (int h = 0; h < 2; h++) {
+                    if (!mbar_wait_warp(s_full(a, h), (done + n) & 1, stop, A.err)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t values = base + S::OFF_RING + s * S::SLOT;
-                    uint32_t any = 0;
-#pragma unroll
-                    for (int i = 0; i < S::SLOT / 16 / 128; i++) {
-                        uint32_t w[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                     : "r"(values + (i * 128 + row) * 16) : "memory");
-                        any |= not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3]);
-                    }
-                    if (any) {
-                        bool found = false;
-#pragma unroll 1
-                        for (int i = row; i < S::SLOT / 16; i += 128) {
-                            const bool inside = p0 + ((i * 16) % S::PANEL) / 128 < it.k1;
-                            uint32_t w[4];
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + i * 16) : "memory");
-                            const bool bad = (not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3])) != 0;
-                            found |= bad && inside;
-                            if (bad || !inside)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * 16), "r"(inside ? finite_part<BF16>(w[0]) : 0u),
-                                             "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
-                                             "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
+                    if (h == 0 && b >= U.clean && (!U.wide || a == 0)) {
+                        // Values that some row may not see must not reach its product as
+                        // 0 * inf, nor may what the slot holds behind the last key: what is
+                        // not finite counts as 0 here, and rows that do see such a value get it
+                        // at the end. (Once S is there the ring has come to this block: its
+                        // slot's phase is not an older one.)
+                        const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
+                        if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
+                            ok = false;
+                            break;
                         }
-                        if (found) *dirty = 1;
-                    }
-                    fence_proxy_async();
-                }
-                tc_fence_after();
-                if (live) {
-                    uint32_t s[128];
-                    tmem_load128_wait(st, s);
-                    if (b >= U.clean) {
-                        const int seen = lim - p0;
+                        const uint32_t values = base + S::OFF_RING + s * S::SLOT;
+                        uint32_t any = 0;
 #pragma unroll
-                        for (int i = 0; i < 128; i++)
-                            if (i >= seen) s[i] = 0xFF800000u;
-                    }
-                    float mx[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) mx[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
-#pragma unroll
-                    for (int i = 8; i < 128; i += 2) mx[(i / 2) & 3] = max3(mx[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-                    const bool grown = top > m + GROWTH;  // also the first maximum: m is -inf before it
-                    if (__any_sync(0xffffffffu, grown)) {
-                        const float f = grown ? exp2_approx(m - top) : 1.0f;
-                        if (grown) m = top;
-                        sum *= f;
-                        if (n > 0) {  // the products up to the previous block are done: this S came after them
+                        for (int i = 0; i < S::SLOT / 16 / 128; i++) {
+                            uint32_t w[4];
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                         : "r"(values + (i * 128 + row) * 16) : "memory");
+                            any |= not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3]);
+                        }
+                        if (any) {
+                            bool found = false;
 #pragma unroll 1
-                            for (int c = 0; c < D; c += 32) {
-                                uint32_t o[32];
-                                tmem_load32_wait(ot + c, o);
+                            for (int i = row; i < S::SLOT / 16; i += 128) {
+                                const bool inside = p0 + ((i * 16) % S::PANEL) / 128 < it.k1;
+                                uint32_t w[4];
+                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + i * 16) : "memory");
+                                const bool bad = (not_finite_bits<BF16>(w[0]) | not_finite_bits<BF16>(w[1]) | not_finite_bits<BF16>(w[2]) | not_finite_bits<BF16>(w[3])) != 0;
+                                found |= bad && inside;
+                                if (bad || !inside)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(values + i * 16), "r"(inside ? finite_part<BF16>(w[0]) : 0u),
+                                                 "r"(inside ? finite_part<BF16>(w[1]) : 0u), "r"(inside ? finite_part<BF16>(w[2]) : 0u),
+                                                 "r"(inside ? finite_part<BF16>(w[3]) : 0u) : "memory");
+                            }
+                            if (found) *dirty = 1;
+                        }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (U.wide && lane == 0) mbar_arrive(v_clean);  // tile 1's products wait for it as well
+                    }
+                    tc_fence_after();
+                    if (live) {
+                        uint32_t s[HALF];
+                        tmem_load64_wait(st + HALF * h, s);
+                        if (b >= U.clean) {
+                            const int seen = lim - p0 - HALF * h;
 #pragma unroll
-                                for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                tmem_store32(ot + c, o);
+                            for (int i = 0; i < HALF; i++)
+                                if (i >= seen) s[i] = 0xFF800000u;
+                        }
+                        float mx[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) mx[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+#pragma unroll
+                        for (int i = 8; i < HALF; i += 2) mx[(i / 2) & 3] = max3(mx[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
+                        const bool grown = top > m + GROWTH;  // also the first maximum: m is -inf before it
+                        if (__any_sync(0xffffffffu, grown)) {
+                            const float f = grown ? exp2_approx(m - top) : 1.0f;
+                            if (grown) m = top;
+                            sum *= f;
+                            if (n > 0 || h > 0) {
+                                // O is still once the previous half's product is done (the one
+                                // before that is: these scores came after it)
+                                if (!mbar_wait_warp(pv_done(a), (h + 1) & 1, stop, A.err)) {
+                                    ok = false;
+                                    break;
+                                }
+                                tc_fence_after();
+#pragma unroll 1
+                                for (int c = 0; c < D; c += 32) {
+                                    uint32_t o[32];
+                                    tmem_load32_wait(ot + c, o);
+#pragma unroll
+                                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                    tmem_store32(ot + c, o);
+                                }
                             }
                         }
-                    }
-                    const float shift = (m == -INFINITY ? 0.0f : -m) + LIFT;
-                    const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
-                    uint64_t sum2[2] = {0, 0};
+                        const float shift = (m == -INFINITY ? 0.0f : -m) + LIFT;
+                        const uint64_t scale2 = pack2(scale, scale), shift2 = pack2(shift, shift);
+                        uint64_t sum2[2] = {0, 0};
+                        uint32_t w[HALF / 2];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const uint64_t x = fma2(pack2u(s[64 * h + 2 * i], s[64 * h + 2 * i + 1]), scale2, shift2);
+                        for (int i = 0; i < HALF / 2; i++) {
+                            const uint64_t x = fma2(pack2u(s[2 * i], s[2 * i + 1]), scale2, shift2);
                             const float e0 = exp2_approx(lo_f(x)), e1 = exp2_approx(hi_f(x));
                             sum2[i & 1] = add2(sum2[i & 1], pack2(e0, e1));
                             w[i] = H::pack(e0, e1);
                         }
-                        tmem_store32(st + 32 * h, w);
-                        if (h == 0) {
-                            tmem_store_wait();
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive(p_half(a));
-                        }
+                        tmem_store32(st + HALF * h, w);
+                        sum2[0] = add2(sum2[0], sum2[1]);
+                        sum += lo_f(sum2[0]) + hi_f(sum2[0]);
+                        tmem_store_wait();
                     }
-                    sum2[0] = add2(sum2[0], sum2[1]);
-                    sum += lo_f(sum2[0]) + hi_f(sum2[0]);
-                    tmem_store_wait();
-                } else if (lane == 0) {
-                    mbar_arrive(p_half(a));
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_full(a, h));
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(p_full(a));
             }
             // ---------------------------------------------------- epilogue
             if (ok && nblocks > 0) ok = mbar_wait_warp(o_full(a), (a ? ends1 : ends0) & 1, stop, A.err);
