@@ -47,6 +47,7 @@ constexpr int TILE_THREADS = 384;
 constexpr int ROWS = 128;      // rows of a tile
 constexpr int BLOCK = 128;     // keys of a block, the step of the ring
 constexpr int HALF = 64;       // keys of one score product: a tile's S has room for two
+constexpr int POLY_EVERY = 4;  // one in this many pairs of weights is computed on the FMA pipe
 constexpr float GROWTH = 8.0f; // log2 of how far a maximum may grow before O is rescaled
 
 template <int D>
@@ -58,7 +59,7 @@ struct TileShape {
     static constexpr int OFF_RING = 2 * SLOT;
     static constexpr int OFF_OUT = OFF_RING + STAGES * SLOT;  // 4 KB per softmax warp: outputs on their way to rows
     static constexpr int OFF_BAR = OFF_OUT + 8 * 4096;
-    static constexpr int OFF_MISC = OFF_BAR + (16 + 2 * STAGES) * 8;
+    static constexpr int OFF_MISC = OFF_BAR + (18 + 2 * STAGES) * 8;
     static constexpr int OFF_JOIN = OFF_MISC + 16;    // (m, sum) of the second tile's rows
     static constexpr int BYTES = OFF_JOIN + ROWS * 8 + 1024;
     static_assert(ROWS * D * 4 == 2 * SLOT, "one tile's f32 outputs take the queries' place");
@@ -152,9 +153,10 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+// The larger of three; NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
 
@@ -195,6 +197,23 @@ struct Unit {
     __device__ __forceinline__ int blocks_of(int tile) const { return wide ? nb : (nb - tile + 1) / 2; }
 };
 
+// 2^x of a pair on the FMA pipe, for x in [-inf, 127): x = n + f with n the
+// nearest integer (adding 1.5 * 2^23 + 127 leaves n + 127 in the sum's low
+// bits), the polynomial that interpolates 2^f at the five Chebyshev nodes of
+// [-1/2, 1/2] (at most 3.6e-6 off, over 400,001 points in f32; the weights are
+// rounded to 2.4e-4 or more), times 2^n. Below -126.5 the result is 0.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    x = pack2(fmaxf(lo_f(x), -127.0f), fmaxf(hi_f(x), -127.0f));
+    const uint64_t t = add2(x, pack2(12583039.0f, 12583039.0f));
+    const uint64_t f = fma2(add2(t, pack2(-12583039.0f, -12583039.0f)), pack2(-1.0f, -1.0f), x);
+    uint64_t p = pack2(0.00966636837f, 0.00966636837f);
+    p = fma2(p, f, pack2(0.0559219755f, 0.0559219755f));
+    p = fma2(p, f, pack2(0.240223497f, 0.240223497f));
+    p = fma2(p, f, pack2(0.693121016f, 0.693121016f));
+    p = fma2(p, f, pack2(1.0f, 1.0f));
+    return mul2(p, pack2u((uint32_t)t << 23, (uint32_t)(t >> 32) << 23));
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_constant__ TileArgs args) {
     using S = TileShape<D>;
@@ -215,8 +234,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     auto pv_done = [&](int a) { return bars + 80 + 8 * a; };  // one phase per half block
     auto o_full = [&](int a) { return bars + 96 + 8 * a; };   // one phase per unit
     const uint32_t v_clean = bars + 112;  // one phase per value block of two tiles that was looked through
-    auto full = [&](int s) { return bars + 128 + 8 * s; };
-    auto empty = [&](int s) { return bars + 128 + 8 * (S::STAGES + s); };
+    auto v_here = [&](int a) { return bars + 120 + 8 * a; };  // one phase per value block that warpgroup a looks through
+    const uint32_t join_ready = bars + 136;                   // one phase per unit whose two tiles are joined
+    auto full = [&](int s) { return bars + 144 + 8 * s; };
+    auto empty = [&](int s) { return bars + 144 + 8 * (S::STAGES + s); };
     uint32_t *const tmem_slot = reinterpret_cast<uint32_t *>(smem + S::OFF_MISC);
     volatile int *const stop = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 4);
     volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);
@@ -229,13 +250,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 mbar_init(p_full(a, h), 4);
             }
             mbar_init(pv_done(a), 1);
+            mbar_init(v_here(a), 1);
             mbar_init(o_full(a), 1);
         }
         for (int s = 0; s < S::STAGES; s++) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), 2);  // one per tile, or twice by the tile whose block it is
+            mbar_init(empty(s), 2);  // one per tile
         }
         mbar_init(v_clean, 4);
+        mbar_init(join_ready, 2);
         mbar_init(q_full, 32);
         mbar_init(q_free, 3);
         *stop = *dirty = 0;
@@ -251,6 +274,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a's half h at 128 a + 64 h, O at 256 + 128 a
 
     const int units = A.plan.counts[COUNT_TILE] * P.kv_heads;  // the host keeps it, and one more round, below 2^31
+    // A barrier only tells the parity of its phase, so whoever waits on one waits
+    // for each of its phases in turn, and none can pass before all who wait have
+    // seen it: every ring slot is released by both tiles, whoever uses it.
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
@@ -272,7 +298,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     const int s = slot % S::STAGES;
                     const int half = lane % S::HALVES, page = lane / S::HALVES, at = b * per + page - window;
                     const int x = __shfl_sync(0xffffffffu, here, at & 31), y = __shfl_sync(0xffffffffu, next, at & 31);
-                    if (!mbar_wait_warp(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
+                    if (!mbar_wait_warp_timed(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
                     const int pages = min(per, npages - b * per);
                     if (lane == 0) mbar_expect_tx(full(s), (uint32_t)pages * P.page_tokens * D * 2);
                     __syncwarp();
@@ -305,6 +331,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             const int a = warp - 9;
             uint32_t ring = 0, turn = 0, done = 0;  // done: key blocks of this tile in earlier units
             uint32_t cleaned = 0;                   // phases of v_clean waited for
+            uint32_t seen = 0;                      // ring slots this tile has been through
             const uint32_t score_desc = idesc_scores<BF16>() | (A.scale_log2 < 0.0f ? NEGATE_A : 0u);
             const uint64_t q_desc = umma_desc_sw128(base), k_desc = umma_desc_sw128(base + S::OFF_RING);
             const uint64_t v_desc = umma_desc_values(base + S::OFF_RING, S::PANEL);
@@ -321,9 +348,25 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 U.clean = uniform(U.clean);
                 const int nblocks = U.blocks_of(a), b0 = U.wide ? 0 : a, step = U.wide ? 1 : 2;
                 const uint64_t qd = q_desc + (U.wide ? a * (S::SLOT >> 4) : 0);
+                // Goes through the ring up to `slot`, releasing at once what is the
+                // other tile's.
+                auto pass = [&](uint32_t slot) {
+                    for (; seen != slot; seen++) {
+                        const uint32_t s = seen % S::STAGES;
+                        if (!mbar_wait_warp_timed(full(s), (seen / S::STAGES) & 1, stop, A.err)) return false;
+                        if (leader) mbar_arrive(empty(s));
+                        __syncwarp();
+                    }
+                    return true;
+                };
+                auto filled = [&](uint32_t slot) {
+                    if (!pass(slot)) return false;
+                    seen++;
+                    return mbar_wait_warp_timed(full(slot % S::STAGES), (slot / S::STAGES) & 1, stop, A.err);
+                };
                 auto scores = [&](int n, int h) {  // of half h of this tile's n-th block
                     const uint32_t slot = U.key_slot(b0 + n * step), s = slot % S::STAGES;
-                    if (h == 0 && !mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    if (h == 0 && !filled(slot)) return false;
                     tc_fence_after();
                     const uint64_t kd = k_desc + s * (S::SLOT >> 4) + h * (HALF * 128 >> 4);
                     if (leader) {
@@ -335,7 +378,6 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                         umma_commit(s_full(a, h));
                         if (h == 1) {
                             umma_commit(empty(s));
-                            if (!U.wide) umma_commit(empty(s));
                             if (n == nblocks - 1) {
                                 // The queries' place is free when both tiles and, where two
                                 // warpgroups join their outputs there, these have said so.
@@ -350,10 +392,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 };
                 auto values = [&](int n, int h) {
                     const uint32_t slot = U.value_slot(b0 + n * step), s = slot % S::STAGES;
-                    if (h == 0 && !mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) return false;
+                    if (h == 0 && !filled(slot)) return false;
                     const uint64_t vd = v_desc + s * (S::SLOT >> 4);
-                    if (h == 0 && a == 1 && U.wide && n >= U.clean && !mbar_wait_warp(v_clean, cleaned++ & 1, stop, A.err)) return false;
-                    if (!mbar_wait_warp(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
+                    const bool masked = h == 0 && b0 + n * step >= U.clean;
+                    if (masked && (!U.wide || a == 0) && leader) mbar_arrive(v_here(a));
+                    __syncwarp();
+                    if (masked && U.wide && a == 1 && !mbar_wait_warp_timed(v_clean, cleaned++ & 1, stop, A.err)) return false;
+                    if (!mbar_wait_warp_timed(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
                     tc_fence_after();
                     if (leader) {
 #pragma unroll
@@ -362,14 +407,16 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                         umma_commit(pv_done(a));
                         if (h == 1) {
                             umma_commit(empty(s));
-                            if (!U.wide) umma_commit(empty(s));
-                            if (n == nblocks - 1) umma_commit(o_full(a));
+                            if (n == nblocks - 1) {
+                                umma_commit(o_full(a));
+                                if (U.two()) umma_commit(join_ready);
+                            }
                         }
                     }
                     __syncwarp();
                     return true;
                 };
-                ok = mbar_wait_warp(q_full, turn & 1, stop, A.err);
+                ok = mbar_wait_warp_timed(q_full, turn & 1, stop, A.err);
                 if (nblocks > 0) ok = ok && scores(0, 0) && scores(0, 1);
                 // A half's next scores follow its weights' product, whose operand they
                 // overwrite; the other half's are there already, so the softmax finds
@@ -379,6 +426,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     for (int h = 0; h < 2; h++) ok = ok && values(n, h) && (n + 1 >= nblocks || scores(n + 1, h));
                 }
                 ring += 2 * U.nb;
+                ok = ok && pass(ring);
                 done += nblocks;
             }
         } else {
@@ -397,7 +445,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     const int rr = U.it.r0 + min(lane + 32 * j, U.it.nr - 1);
                     off[j] = A.plan.perm[U.it.tok0 + rr / A.group] * A.q_stride + (U.kvh * A.group + rr % A.group) * D;
                 }
-                ok = mbar_wait_warp(q_free, (turn & 1) ^ 1, stop, A.err);
+                ok = mbar_wait_warp_timed(q_free, (turn & 1) ^ 1, stop, A.err);
                 if (!ok) break;
                 const int c = lane % VEC;
                 const uint32_t dst = base + (c >> 3) * S::PANEL;
@@ -428,7 +476,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
         const uint32_t st = tmem + lanes + 128 * a, ot = tmem + lanes + 256 + 128 * a;
         uint32_t ring = 0, turn = 0;
         uint32_t done = 0;          // key blocks of this tile in earlier units
-        uint32_t ends0 = 0, ends1 = 0;  // earlier units in which each tile had a block
+        uint32_t ends = 0;          // earlier units in which this tile had a block
+        uint32_t joins = 0;         // earlier units whose tiles were joined
+        uint32_t looked = 0;        // value blocks looked through
         bool ok = true;  // false once a wait gave up: the remaining units' barriers are still met
         for (int i = 0; i * (int)gridDim.x < units; i++, turn++) {
             if (dealt(i) >= units) break;
@@ -449,7 +499,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
 #pragma unroll 1
                 for (int h = 0; h < 2; h++) {
-                    if (!mbar_wait_warp(s_full(a, h), (done + n) & 1, stop, A.err)) {
+                    if (!mbar_wait_warp_timed(s_full(a, h), (done + n) & 1, stop, A.err)) {
                         ok = false;
                         break;
                     }
@@ -457,10 +507,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                         // Values that some row may not see must not reach its product as
                         // 0 * inf, nor may what the slot holds behind the last key: what is
                         // not finite counts as 0 here, and rows that do see such a value get it
-                        // at the end. (Once S is there the ring has come to this block: its
-                        // slot's phase is not an older one.)
-                        const uint32_t slot = U.value_slot(b), s = slot % S::STAGES;
-                        if (!mbar_wait_warp(full(s), (slot / S::STAGES) & 1, stop, A.err)) {
+                        // at the end.
+                        const uint32_t s = U.value_slot(b) % S::STAGES;
+                        if (!mbar_wait_warp_timed(v_here(a), looked++ & 1, stop, A.err)) {
                             ok = false;
                             break;
                         }
@@ -505,19 +554,21 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                         }
                         float mx[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) mx[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+                        for (int i = 0; i < 4; i++) mx[i] = max3(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]), -INFINITY);
 #pragma unroll
                         for (int i = 8; i < HALF; i += 2) mx[(i / 2) & 3] = max3(mx[(i / 2) & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale;
-                        const bool grown = top > m + GROWTH;  // also the first maximum: m is -inf before it
+                        const float top = max3(max3(mx[0], mx[1], mx[2]), mx[3], -INFINITY) * scale;
+                        // also the first maximum (m is -inf before it), and a score that is not a
+                        // number: m and with it the row's sum become NaN, as for one of +inf
+                        const bool grown = !(top <= m + GROWTH);
                         if (__any_sync(0xffffffffu, grown)) {
                             const float f = grown ? exp2_approx(m - top) : 1.0f;
-                            if (grown) m = top;
+                            if (grown) m = top < INFINITY ? top : __int_as_float(0x7FC00000);
                             sum *= f;
                             if (n > 0 || h > 0) {
                                 // O is still once the previous half's product is done (the one
                                 // before that is: these scores came after it)
-                                if (!mbar_wait_warp(pv_done(a), (h + 1) & 1, stop, A.err)) {
+                                if (!mbar_wait_warp_timed(pv_done(a), (h + 1) & 1, stop, A.err)) {
                                     ok = false;
                                     break;
                                 }
@@ -539,9 +590,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
 #pragma unroll
                         for (int i = 0; i < HALF / 2; i++) {
                             const uint64_t x = fma2(pack2u(s[2 * i], s[2 * i + 1]), scale2, shift2);
-                            const float e0 = exp2_approx(lo_f(x)), e1 = exp2_approx(hi_f(x));
-                            sum2[i & 1] = add2(sum2[i & 1], pack2(e0, e1));
-                            w[i] = H::pack(e0, e1);
+                            // some on the FMA pipe: the exponential unit is the scarcer one
+                            const uint64_t e = i % POLY_EVERY == POLY_EVERY - 1 ? exp2_poly(x) : pack2(exp2_approx(lo_f(x)), exp2_approx(hi_f(x)));
+                            sum2[i & 1] = add2(sum2[i & 1], e);
+                            w[i] = H::pack(lo_f(e), hi_f(e));
                         }
                         tmem_store32(st + HALF * h, w);
                         sum2[0] = add2(sum2[0], sum2[1]);
@@ -554,13 +606,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
             }
             // ---------------------------------------------------- epilogue
-            if (ok && nblocks > 0) ok = mbar_wait_warp(o_full(a), (a ? ends1 : ends0) & 1, stop, A.err);
+            if (ok && nblocks > 0) ok = mbar_wait_warp_timed(o_full(a), ends & 1, stop, A.err);
             const bool two = U.two();
             if (two) {
                 if (a == 1) {
                     // no product reads the queries any more once tile 0 is done too:
                     // their place takes this tile's outputs, [dim][row]
-                    if (ok) ok = mbar_wait_warp(o_full(0), ends0 & 1, stop, A.err);
+                    if (ok) ok = mbar_wait_warp_timed(join_ready, joins & 1, stop, A.err);
                     if (ok && live) {
                         tc_fence_after();
 #pragma unroll 1
@@ -655,8 +707,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             tc_fence_before();
             ring += 2 * U.nb;
             done += nblocks;
-            ends0++;
-            ends1 += U.blocks_of(1) > 0;
+            ends += nblocks > 0;
+            joins += two;
             if (two) {  // the joined outputs have been read: their place is free
                 asm volatile("bar.sync 2, 256;" ::: "memory");
                 if (threadIdx.x == 0) mbar_arrive(q_free);

@@ -85,6 +85,26 @@ __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, vo
     }
 }
 
+// As mbar_wait_warp, bounded by time: about 2 s of SM clock.
+__device__ __forceinline__ bool mbar_wait_warp_timed(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+    const long long t0 = clock64();
+    for (uint32_t i = 0;; i++) {
+        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+        if ((i & 63) == 63) {
+            int stop = *abort_flag ? 1 : (clock64() - t0 > 4000000000LL ? 2 : 0);
+            stop = __shfl_sync(0xffffffffu, stop, 0);
+            if (stop) {
+                if (stop == 2 && (threadIdx.x & 31) == 0) {
+                    *abort_flag = 1;
+                    if (err) atomicExch(err, 3);
+                }
+                return false;
+            }
+        }
+    }
+}
+
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
