@@ -197,6 +197,7 @@ class ShieldContext:
 
     def __init__(self, device_mask: int = 1):
         self._h = C.c_void_p()
+        self._page_tokens = {}  # of each paged cache
         _check(lib().shield_open(device_mask, C.byref(self._h)))
 
     def close(self):
@@ -332,6 +333,7 @@ class ShieldContext:
         c = ShieldKvConfig(_KV_TYPES[type], n_layers, n_kv_heads, head_dim, page_tokens, n_pages, k, v)
         out = C.c_int64()
         _check(lib().shield_kv_create(self._h, device, C.byref(c), C.byref(out)))
+        self._page_tokens[out.value] = page_tokens
         return out.value
 
     def kv_release(self, kv: int) -> None:
@@ -392,7 +394,7 @@ class ShieldContext:
     def kv_pages(self, kv: int, seqs) -> np.ndarray:
         """The sequences' page numbers, one row each, padded with -1."""
         s = np.ascontiguousarray(seqs, np.int64)
-        most = -(-int(self.kv_lengths(kv, s).max(initial=0)) // self.kv_info(kv)["page_tokens"])
+        most = -(-int(self.kv_lengths(kv, s).max(initial=0)) // self._page_tokens.get(kv, 1))
         out = np.empty((s.size, most), np.int32)
         _check(lib().shield_kv_pages(self._h, kv, _addr(s), s.size, None, _addr(out), most))
         return out

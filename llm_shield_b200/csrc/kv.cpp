@@ -115,6 +115,8 @@ static void create(shield_ctx *ctx, int32_t device, const shield_kv_config *cfg,
         SHIELD_CUDA(cudaMalloc(&P.k, (size_t)P.layer_stride() * P.layers * 2));
         SHIELD_CUDA(cudaMalloc(&P.v, (size_t)P.layer_stride() * P.layers * 2));
     }
+    if (!map_pool(&cache->maps[0], P, P.k) || !map_pool(&cache->maps[1], P, P.v))
+        throw Error(SHIELD_ERR_CUDA, "the pool's memory cannot be mapped for TMA");
     S.caches.emplace(id, std::move(cache));
     S.next_cache++;
     *out = id;
@@ -174,7 +176,7 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     const size_t o_counts = place(COUNTS, 4), o_few = place((size_t)S.max_items, sizeof(Item)),
                  o_tile = place((size_t)S.max_items, sizeof(Item)), o_segs = place((size_t)S.max_segments, sizeof(Segment)),
                  o_slot = place((size_t)T, 4), o_perm = place((size_t)T, 4), o_lim = place((size_t)T, 4),
-                 o_leaf = place((size_t)T, 4), o_merge = place((size_t)T, 4), o_where = place((size_t)S.max_items, 4),
+                 o_merge = place((size_t)T, sizeof(Join)), o_where = place((size_t)S.max_items, 4),
                  o_table = place((size_t)S.max_table, 4);
     B->bytes = at;
     SHIELD_CUDA(cudaMalloc(&B->dev, at));
@@ -196,8 +198,7 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     P.slot = ints(o_slot);
     P.perm = ints(o_perm);
     P.lim = ints(o_lim);
-    P.leaf = ints(o_leaf);
-    P.merge = ints(o_merge);
+    P.merge = reinterpret_cast<const Join *>(B->dev + o_merge);
     P.where = ints(o_where);
     P.table = ints(o_table);
     P.part_o = B->part_o;
@@ -263,8 +264,7 @@ static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const
     send(P.slot, plan.slot.data(), plan.slot.size() * 4);
     send(P.perm, plan.perm.data(), plan.perm.size() * 4);
     send(P.lim, plan.lim.data(), plan.lim.size() * 4);
-    send(P.leaf, plan.leaf.data(), plan.leaf.size() * 4);
-    send(P.merge, plan.merge.data(), plan.merge.size() * 4);
+    send(P.merge, plan.merge.data(), plan.merge.size() * sizeof(Join));
     send(P.where, plan.where.data(), plan.where.size() * 4);
     send(P.table, plan.table.data(), plan.table.size() * 4);
     SHIELD_CUDA(cudaEventRecord(B.sent[turn], s));
@@ -352,7 +352,7 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     const int64_t few = cap ? 2 * (int64_t)c.dev.sms : (int64_t)B.last.few.size() * c.pool.kv_heads;
     const int64_t tile = cap ? (int64_t)c.dev.sms : (int64_t)B.last.tile.size() * c.pool.kv_heads;
     const int64_t join = cap ? std::min<int64_t>(B.max_tokens, 4096) : (int64_t)B.last.merge.size();
-    check(launch_attend_tile(A, tile, c.dev.sms, s), "attention, many rows");
+    check(launch_attend_tile(A, c.maps, tile, c.dev.sms, s), "attention, many rows");
     check(launch_attend_few(A, few, s), "attention, few rows");
     check(launch_attend_merge(A, join, s), "attention, joining");
 }

@@ -16,6 +16,7 @@ struct Cache {
     int64_t id = 0;
     DeviceView dev;
     DevPool pool;
+    CUtensorMap maps[2];  // keys, values
     Pool book;
     bool owns = false;  // the pool's memory is the library's
     Cache(const Pool &b) : book(b) {}

@@ -263,7 +263,8 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
 template <bool BF16, int D>
 static cudaError_t few_launch(const AttendArgs &A, int64_t units, cudaStream_t s) {
     using S = FewShape<D>;
-    cudaError_t e = cudaFuncSetAttribute(k_attend_few<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(k_attend_few<BF16, D>, S::BYTES, allowed);
     if (e != cudaSuccess) return e;
     k_attend_few<BF16, D><<<(unsigned)std::min<int64_t>(units, 1 << 30), 128, S::BYTES, s>>>(A);
     return cudaGetLastError();
@@ -278,8 +279,10 @@ cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s
 
 // ----------------------------------------------------------------- joining
 
-// One warp per (token, query head): the row's partials, from its sequence's
-// own keys up through the runs it shares, always in that order.
+// One warp per (token, query head). The row's partials lie one per piece of
+// keys of each segment on the way from the sequence's own keys up through the
+// runs it shares, always in that order. A lane looks up one piece, so that the
+// lookups of up to 32 pieces and the reads of their outputs go out together.
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
     using H = Half16<BF16>;
@@ -288,32 +291,60 @@ __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
     const int heads = A.group * A.pool.kv_heads;
     const int64_t rows = (int64_t)A.plan.counts[COUNT_MERGE] * heads;
     for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < rows; w += (int64_t)gridDim.x * 4) {
-        const int at = A.plan.merge[w / heads], head = (int)(w % heads), kvh = head / A.group;
+        const Join J = A.plan.merge[w / heads];
+        const int head = (int)(w % heads), kvh = head / A.group;
         float M = -INFINITY, L = 0.0f, o[E];
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = 0.0f;
-        for (int sg = A.plan.leaf[at]; sg >= 0;) {
+        for (int sg = J.leaf; sg >= 0;) {
             const Segment S = A.plan.segs[sg];
-            const int r = (at - S.tok0) * A.group + head % A.group, tile = r / S.tile_rows;
-            for (int sp = 0; sp < S.nsplit; sp++) {
-                const int item = A.plan.where[S.item0 + sp * S.ntiles + tile];
-                if (item < 0) continue;
-                const Item *it = (S.tile_kind ? A.plan.tile : A.plan.few) + item;
-                const int64_t part = it->part + (int64_t)kvh * it->nr + (r - it->r0);
-                const float2 ml = A.plan.part_ml[part];
-                const float mn = fmaxf(M, ml.x), ref = mn == -INFINITY ? 0.0f : mn;
-                const float a = exp2_approx(M - ref), b = exp2_approx(ml.x - ref);
-                M = mn;
-                L = __fmaf_rn(ml.y, b, L * a);
+            const int r = (J.at - S.tok0) * A.group + head % A.group, tile = r / S.tile_rows, in_tile = r % S.tile_rows;
+            const int nr = min(S.tile_rows, S.rows - tile * S.tile_rows);
+            for (int s0 = 0; s0 < S.nsplit; s0 += 32) {
+                const int n = min(32, S.nsplit - s0);
+                int part = lane < n ? A.plan.where[S.slot0 + (s0 + lane) * S.ntiles + tile] : -1;
+                float2 ml = make_float2(-INFINITY, 0.0f);
+                if (part >= 0) {
+                    part += kvh * nr + in_tile;
+                    ml = A.plan.part_ml[part];
+                }
+                float top = ml.x;
 #pragma unroll
-                for (int e = 0; e < E; e++) o[e] = __fmaf_rn(A.plan.part_o[part * D + lane * E + e], b, o[e] * a);
+                for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float mn = fmaxf(M, top), ref = mn == -INFINITY ? 0.0f : mn;
+                const float old = exp2_approx(M - ref), f = exp2_approx(ml.x - ref);
+                M = mn;
+                float l = ml.y * f;
+#pragma unroll
+                for (int d = 16; d > 0; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+                L = __fmaf_rn(L, old, l);
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] *= old;
+#pragma unroll 8
+                for (int s = 0; s < n; s++) {
+                    const int p = __shfl_sync(0xffffffffu, part, s);
+                    const float g = __shfl_sync(0xffffffffu, f, s);
+                    if (p < 0) continue;
+                    const float *src = A.plan.part_o + (int64_t)p * D + lane * E;
+                    if constexpr (E == 4) {
+                        const float4 x = *reinterpret_cast<const float4 *>(src);
+                        o[0] = __fmaf_rn(x.x, g, o[0]);
+                        o[1] = __fmaf_rn(x.y, g, o[1]);
+                        o[2] = __fmaf_rn(x.z, g, o[2]);
+                        o[3] = __fmaf_rn(x.w, g, o[3]);
+                    } else {
+                        const float2 x = *reinterpret_cast<const float2 *>(src);
+                        o[0] = __fmaf_rn(x.x, g, o[0]);
+                        o[1] = __fmaf_rn(x.y, g, o[1]);
+                    }
+                }
             }
             sg = S.parent;
         }
         const float inv = 1.0f / L;
-        uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + lane * E;
-#pragma unroll
-        for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t *>(out + e) = H::pack(o[e] * inv, o[e + 1] * inv);
+        uint16_t *out = static_cast<uint16_t *>(A.out) + J.token * A.out_stride + head * D + lane * E;
+        if constexpr (E == 4) *reinterpret_cast<uint2 *>(out) = make_uint2(H::pack(o[0] * inv, o[1] * inv), H::pack(o[2] * inv, o[3] * inv));
+        else *reinterpret_cast<uint32_t *>(out) = H::pack(o[0] * inv, o[1] * inv);
     }
 }
 

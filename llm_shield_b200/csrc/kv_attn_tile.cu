@@ -742,7 +742,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-static bool map_pool(CUtensorMap *m, const DevPool &P, void *data) {
+bool map_pool(CUtensorMap *m, const DevPool &P, void *data) {
     auto fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t row = (cuuint64_t)P.dim * 2;
@@ -758,17 +758,19 @@ static bool map_pool(CUtensorMap *m, const DevPool &P, void *data) {
 template <bool BF16, int D>
 static cudaError_t tile_launch(const TileArgs &T, int64_t units, int sms, cudaStream_t s) {
     using S = TileShape<D>;
-    cudaError_t e = cudaFuncSetAttribute(k_attend_tile<BF16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(k_attend_tile<BF16, D>, S::BYTES, allowed);
     if (e != cudaSuccess) return e;
     k_attend_tile<BF16, D><<<(unsigned)std::min<int64_t>(units, sms), TILE_THREADS, S::BYTES, s>>>(T);
     return cudaGetLastError();
 }
 
-cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, int sms, cudaStream_t s) {
+cudaError_t launch_attend_tile(const AttendArgs &A, const CUtensorMap *maps, int64_t units, int sms, cudaStream_t s) {
     if (units == 0) return cudaSuccess;
     TileArgs T;
     T.a = A;
-    if (!map_pool(&T.k, A.pool, A.pool.k) || !map_pool(&T.v, A.pool, A.pool.v)) return cudaErrorInvalidValue;
+    T.k = maps[0];
+    T.v = maps[1];
     if (A.pool.dim == 128) return A.pool.bf16 ? tile_launch<true, 128>(T, units, sms, s) : tile_launch<false, 128>(T, units, sms, s);
     if (A.pool.dim == 64) return A.pool.bf16 ? tile_launch<true, 64>(T, units, sms, s) : tile_launch<false, 64>(T, units, sms, s);
     return cudaErrorInvalidValue;

@@ -5,6 +5,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "kv_ops.h"
 
 namespace shield {
@@ -66,6 +68,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Lets a kernel use `bytes` of shared memory, once per device (`done`: a bit for
+// each of the first 64; calls from several host threads set the same).
+template <class K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
 // First element of position `row` of a page: layer, page, kv head.
 __device__ __forceinline__ int64_t row_offset(const DevPool &P, int layer, int page, int head, int row) {
     return (int64_t)layer * P.layer_stride() +

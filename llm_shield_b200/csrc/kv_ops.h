@@ -2,6 +2,7 @@
 // Every launcher is asynchronous on the given stream and allocates nothing.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -24,8 +25,8 @@ struct DevPool {
 // reads whatever plan was uploaded last.
 struct DevPlan {
     const int32_t *counts = nullptr;  // tokens, few items, tile items, tokens to join
-    const int32_t *slot = nullptr, *perm = nullptr, *lim = nullptr, *leaf = nullptr, *where = nullptr, *merge = nullptr,
-                  *table = nullptr;
+    const int32_t *slot = nullptr, *perm = nullptr, *lim = nullptr, *where = nullptr, *table = nullptr;
+    const Join *merge = nullptr;
     const Segment *segs = nullptr;
     const Item *few = nullptr, *tile = nullptr;
     float *part_o = nullptr;   // [partial row][dim], not divided by the row's sum
@@ -54,7 +55,9 @@ cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t 
 // The three attention kernels over `units` work units (or as many as a later
 // plan may have: each strides over the plan's own count).
 cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s);
-cudaError_t launch_attend_tile(const AttendArgs &A, int64_t units, int sms, cudaStream_t s);  // one persistent CTA per SM
+// maps: map_pool of the keys and of the values, made once per pool.
+bool map_pool(CUtensorMap *m, const DevPool &pool, void *data);
+cudaError_t launch_attend_tile(const AttendArgs &A, const CUtensorMap *maps, int64_t units, int sms, cudaStream_t s);  // one persistent CTA per SM
 cudaError_t launch_attend_merge(const AttendArgs &A, int64_t tokens, cudaStream_t s);
 
 }  // namespace kv

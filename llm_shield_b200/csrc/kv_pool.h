@@ -221,10 +221,17 @@ struct Item {
 };
 
 // Keys that a set of tokens attends to together: a run of pages that several
-// sequences share, or (a leaf) the rest of one sequence. Its items are
-// where[item0 + split * ntiles + tile], each of tile_rows rows.
+// sequences share, or (a leaf) the rest of one sequence. Its rows (tokens times
+// query heads of a kv head) are cut into ntiles tiles of tile_rows, its keys
+// into nsplit pieces; the item of piece s and tile t has its partial rows from
+// where[slot0 + s * ntiles + t] on (-1: it has none).
 struct Segment {
-    int32_t tok0, item0, ntiles, nsplit, tile_rows, parent, direct, tile_kind;
+    int32_t tok0, rows, slot0, ntiles, nsplit, tile_rows, parent, direct;
+};
+// A token whose rows are joined from partials: its place in plan order, its
+// batch token and its leaf segment.
+struct Join {
+    int32_t at, token, leaf;
 };
 
 struct PlanShape {
@@ -240,15 +247,15 @@ struct PlanShape {
 
 struct Plan {
     std::vector<int32_t> slot;             // per batch token: page * page_tokens + row, where its key and value go
-    std::vector<int32_t> perm, lim, leaf;  // per token in plan order: batch token, visible keys, its leaf segment
+    std::vector<int32_t> perm, lim;        // per token in plan order: batch token, visible keys
     std::vector<Segment> segs;
     std::vector<Item> few, tile;           // longest first
-    std::vector<int32_t> where;            // item of each segment slot, in few or tile; -1: no keys
-    std::vector<int32_t> merge;            // plan-order tokens whose rows are joined from partials
+    std::vector<int32_t> where;            // first partial row of each segment slot, -1: none
+    std::vector<Join> merge;
     std::vector<int32_t> table;
     int64_t part_rows = 0;
     void clear() {
-        slot.clear(); perm.clear(); lim.clear(); leaf.clear(); segs.clear(); few.clear(); tile.clear(); where.clear(); merge.clear();
+        slot.clear(); perm.clear(); lim.clear(); segs.clear(); few.clear(); tile.clear(); where.clear(); merge.clear();
         table.clear();
         part_rows = 0;
     }
@@ -300,6 +307,7 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
     };
     std::vector<Node> stack;
     std::vector<Draft> drafts;
+    std::vector<int32_t> leaf;  // of each token in plan order
     {
         Node root{{}, 0, 0, -1};
         for (int32_t i = 0; i < (int32_t)mem.size(); i++) root.members.push_back(i);
@@ -331,7 +339,7 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
             for (int32_t j = 0; j < first.count; j++) {
                 P.perm.push_back(first.tok + j);
                 P.lim.push_back(len - first.count + j + 1);
-                P.leaf.push_back((int32_t)drafts.size());
+                leaf.push_back((int32_t)drafts.size());
             }
             drafts.push_back({t0, first.count, nd.start * pt, len, first.table, nd.parent, true});
             continue;
@@ -367,15 +375,12 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
         }
         stack.push_back(std::move(next));
     }
-    // How long a piece may be: every SM gets about as many keys to work on.
-    int64_t few_keys = 0, tile_steps = 0;
+    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
     auto is_few = [&](const Draft &d) { return (int64_t)d.ntok * G <= S.few_rows; };
+    auto steps_of = [&](const Draft &d) { return up(d.k1 - d.k0, KEY_STEP); };
     int64_t wide_units = 0;
-    for (const Draft &d : drafts) {
-        const int64_t rows = (int64_t)d.ntok * G;
-        if (is_few(d)) few_keys += (int64_t)(d.k1 - d.k0) * ((rows + FEW_TILE - 1) / FEW_TILE);
-        else wide_units += (rows + 255) / 256;
-    }
+    for (const Draft &d : drafts)
+        if (!is_few(d)) wide_units += up((int64_t)d.ntok * G, 256);
     // 256-row tiles share each key block between two row blocks; 128-row ones
     // when 256-row ones would leave SMs idle
     const int32_t wide = wide_units * S.kv_heads < S.sms ? 128 : 256;
@@ -383,17 +388,40 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
         if (is_few(d)) return FEW_TILE;
         return (int64_t)d.ntok * G <= 128 ? 128 : wide;
     };
-    for (const Draft &d : drafts)
-        if (!is_few(d)) {
-            const int64_t rows = (int64_t)d.ntok * G;
-            tile_steps += (int64_t)((d.k1 - d.k0 + KEY_STEP - 1) / KEY_STEP) * ((rows + tile_rows(d) - 1) / tile_rows(d));
+    // How many steps of keys a piece may have: of the lengths tried, the one with
+    // the least estimated time on `slots` places that work side by side. Up to a
+    // few rounds of pieces the rounds count, each as long as a longest piece and
+    // `extra` steps for its start and end; beyond that the sum.
+    auto piece_steps = [&](bool few, int64_t slots, int64_t extra, int64_t least) {
+        int64_t longest = 0;
+        for (const Draft &d : drafts)
+            if (is_few(d) == few) longest = std::max(longest, steps_of(d));
+        if (longest <= least || !split) return std::max<int64_t>(longest, 1);
+        int64_t best = longest;
+        double best_time = 1e300;
+        for (int64_t n = 1; n <= std::min<int64_t>(longest / least + 1, 64); n++) {
+            const int64_t c = std::max(least, up(longest, n));
+            int64_t units = 0, work = 0;
+            for (const Draft &d : drafts)
+                if (is_few(d) == few) {
+                    const int64_t tiles = up((int64_t)d.ntok * G, tile_rows(d)), pieces = up(steps_of(d), c);
+                    units += tiles * pieces * S.kv_heads;
+                    work += tiles * S.kv_heads * (steps_of(d) + pieces * extra);
+                }
+            const double sum = (double)work / (double)slots + 0.5 * (double)(c + extra);
+            const double rounds = (double)up(units, slots) * (double)(c + extra);
+            const double time = std::max((double)(c + extra), units <= 4 * slots ? std::min(rounds, 2 * sum) : sum) + (n > 1 ? 1.0 : 0.0);
+            if (time < best_time - 1e-9) {
+                best_time = time;
+                best = c;
+            }
         }
-    auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-    const int64_t few_chunk = std::max<int64_t>(2, up(up(few_keys * S.kv_heads, (int64_t)S.sms * 4), KEY_STEP)) * KEY_STEP;
-    const int64_t tile_chunk = std::max<int64_t>(4, up(tile_steps * S.kv_heads, S.sms)) * KEY_STEP;
+        return best;
+    };
+    const int64_t few_chunk = piece_steps(true, (int64_t)S.sms * 2, 3, 4) * KEY_STEP;
+    const int64_t tile_chunk = piece_steps(false, S.sms, 4, 4) * KEY_STEP;
     struct Ref {
         int64_t cost;
-        int32_t slot;
         Item it;
         bool few;
     };
@@ -403,13 +431,13 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
         const int64_t rows = (int64_t)d.ntok * G, keys = d.k1 - d.k0;
         const bool few = is_few(d);
         sg.tok0 = d.tok0;
-        sg.item0 = (int32_t)P.where.size();
+        sg.rows = (int32_t)rows;
+        sg.slot0 = (int32_t)P.where.size();
         sg.tile_rows = tile_rows(d);
         sg.ntiles = (int32_t)up(rows, sg.tile_rows);
         sg.nsplit = split ? (int32_t)up(keys, few ? few_chunk : tile_chunk) : 1;
         sg.parent = d.parent;
         sg.direct = d.leaf && d.parent < 0 && sg.nsplit == 1;
-        sg.tile_kind = !few;
         const int64_t step = up(up(keys, sg.nsplit), KEY_STEP) * KEY_STEP;
         if ((int64_t)P.where.size() + (int64_t)sg.nsplit * sg.ntiles > S.max_items) return false;
         for (int32_t sp = 0; sp < sg.nsplit; sp++)
@@ -437,20 +465,16 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
                     if (P.part_rows > S.max_part) return false;
                 }
                 const int64_t cost = (int64_t)((it.k1 - it.k0 + KEY_STEP - 1) / KEY_STEP) * (it.nr > 128 ? 2 : 1);
-                refs.push_back({cost, (int32_t)P.where.size(), it, few});
-                P.where.push_back(-1);
+                refs.push_back({cost, it, few});
+                P.where.push_back(it.part);
             }
         P.segs.push_back(sg);
     }
     if ((int64_t)P.segs.size() > S.max_segments) return false;
     std::stable_sort(refs.begin(), refs.end(), [](const Ref &a, const Ref &b) { return a.cost > b.cost; });
-    for (const Ref &r : refs) {
-        std::vector<Item> &list = r.few ? P.few : P.tile;
-        P.where[r.slot] = (int32_t)list.size();
-        list.push_back(r.it);
-    }
+    for (const Ref &r : refs) (r.few ? P.few : P.tile).push_back(r.it);
     for (int32_t t = 0; t < (int32_t)P.perm.size(); t++)
-        if (!P.segs[P.leaf[t]].direct) P.merge.push_back(t);
+        if (!P.segs[leaf[t]].direct) P.merge.push_back({t, P.perm[t], leaf[t]});
     return true;
 }
 

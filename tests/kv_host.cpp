@@ -68,7 +68,7 @@ int32_t host_plan(Host *h, const int64_t *ids, const int32_t *c, int32_t n, int3
     });
     return rc ? rc : fits ? 0 : -1;
 }
-// which: 0 slot, 1 perm, 2 lim, 3 leaf, 4 segs, 5 few, 6 tile, 7 where, 8 merge, 9 table; returns int32 words
+// which: 0 slot, 1 perm, 2 lim, 3 merge, 4 segs, 5 few, 6 tile, 7 where, 8 table; returns int32 words
 int64_t host_plan_array(Host *h, int32_t which, int32_t *out) {
     const Plan &P = h->plan;
     auto give = [&](const void *p, size_t words) {
@@ -79,13 +79,12 @@ int64_t host_plan_array(Host *h, int32_t which, int32_t *out) {
     case 0: return give(P.slot.data(), P.slot.size());
     case 1: return give(P.perm.data(), P.perm.size());
     case 2: return give(P.lim.data(), P.lim.size());
-    case 3: return give(P.leaf.data(), P.leaf.size());
+    case 3: return give(P.merge.data(), P.merge.size() * sizeof(Join) / 4);
     case 4: return give(P.segs.data(), P.segs.size() * sizeof(Segment) / 4);
     case 5: return give(P.few.data(), P.few.size() * sizeof(Item) / 4);
     case 6: return give(P.tile.data(), P.tile.size() * sizeof(Item) / 4);
     case 7: return give(P.where.data(), P.where.size());
-    case 8: return give(P.merge.data(), P.merge.size());
-    case 9: return give(P.table.data(), P.table.size());
+    case 8: return give(P.table.data(), P.table.size());
     }
     return -1;
 }

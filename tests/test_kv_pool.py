@@ -101,8 +101,8 @@ class HostPool:
             return None
         self.check(rc)
         get = {}
-        for k, (name, width) in enumerate([("slot", 1), ("perm", 1), ("lim", 1), ("leaf", 1), ("segs", 8), ("few", 8),
-                                           ("tile", 8), ("where", 1), ("merge", 1), ("table", 1)]):
+        for k, (name, width) in enumerate([("slot", 1), ("perm", 1), ("lim", 1), ("merge", 3), ("segs", 8), ("few", 8),
+                                           ("tile", 8), ("where", 1), ("table", 1)]):
             a = np.empty(self.L.host_plan_array(self.h, k, None), np.int32)
             self.L.host_plan_array(self.h, k, a.ctypes.data)
             get[name] = a if width == 1 else a.reshape(-1, width)
@@ -250,38 +250,34 @@ def check_plan(H, ids, counts, P, group, kv_heads):
     assert (P["lim"] == pos[P["perm"]] + 1).all()
     seen = [np.zeros((group, p + 1), np.int8) for p in pos]  # per token in batch order
     part_used = np.zeros(P["part_rows"], np.int8)
-    at_item = {}
-    for s, sg in enumerate(P["segs"].tolist()):
-        tok0, item0, ntiles, nsplit, tile_rows, parent, direct, kind = sg
-        assert parent < s
+    segs = P["segs"].tolist()
+    of_part = {}  # first partial row -> (segment, split, tile)
+    for s, (tok0, rows, slot0, ntiles, nsplit, tile_rows, parent, direct) in enumerate(segs):
+        assert parent < s and ntiles == -(-rows // tile_rows) and (not direct or (parent == -1 and nsplit == 1))
         for sp in range(nsplit):
             for t in range(ntiles):
-                w = int(P["where"][item0 + sp * ntiles + t])
+                w = int(P["where"][slot0 + sp * ntiles + t])
                 if w >= 0:
-                    key = (kind, w)
-                    assert key not in at_item
-                    at_item[key] = (s, sp, t)
-    assert len(at_item) == len(P["few"]) + len(P["tile"])
+                    assert w not in of_part and not direct
+                    of_part[w] = (s, sp, t)
+    inside = {}  # token in plan order -> segments whose pieces hold its rows
     for kind, name in ((0, "few"), (1, "tile")):
         cost = None
-        for w, it in enumerate(P[name].tolist()):
+        for it in P[name].tolist():
             tok0, r0, nr, k0, k1, table, part, masked = it
-            s, sp, t = at_item[kind, w]
-            sg = P["segs"][s].tolist()
-            assert sg[0] == tok0 and r0 == t * sg[4] and 1 <= nr <= sg[4] <= 256 and sg[7] == kind
-            if kind == 0:
-                assert nr <= FEW_TILE
+            assert 1 <= nr <= (FEW_TILE if kind == 0 else 256)
             assert 0 <= k0 < k1 and k0 % pt == 0
             blocks = -(-(k1 - k0) // 128) * (2 if nr > 128 else 1)
             assert cost is None or blocks <= cost  # longest first
             cost = blocks
-            if sg[6]:
-                assert part == -1
-            else:
-                assert part >= 0
+            if part >= 0:
+                s, sp, t = of_part.pop(part)
+                assert segs[s][0] == tok0 and r0 == t * segs[s][5] and nr == min(segs[s][5], segs[s][1] - r0)
                 rows = part_used[part:part + nr * kv_heads]
                 assert rows.size == nr * kv_heads and not rows.any()
                 rows[:] = 1
+                for t in range(tok0 + r0 // group, tok0 + (r0 + nr - 1) // group + 1):
+                    inside.setdefault(t, set()).add(s)
             first = int(P["lim"][tok0 + r0 // group])
             for r in range(r0, r0 + nr):
                 tok = int(P["perm"][tok0 + r // group])
@@ -290,28 +286,26 @@ def check_plan(H, ids, counts, P, group, kv_heads):
                 if not masked:
                     assert lim >= k1
                 own = pages[owner[tok]]
-                assert P["table"][table + k0 // pt:table + (k1 - 1) // pt + 1].tolist()[:len(range(k0 // pt, (min(lim, k1) - 1) // pt + 1))] == \
-                    own[k0 // pt:(min(lim, k1) - 1) // pt + 1] if lim > k0 else True
+                last = (min(lim, k1) - 1) // pt + 1
+                if lim > k0:
+                    assert P["table"][table + k0 // pt:table + last].tolist() == own[k0 // pt:last]
                 assert table + (k1 - 1) // pt < P["table"].size
                 row = seen[tok][r % group]
                 assert not row[k0:min(k1, lim)].any()
                 row[k0:min(k1, lim)] = 1
-    assert part_used.all()
+    assert part_used.all() and not of_part
     for tok in range(T):
         assert seen[tok].all()
-    direct = {t for t in range(T) if P["segs"][P["leaf"][t]][6]}
-    assert sorted(P["merge"].tolist()) == [t for t in range(T) if t not in direct]
-    for t in direct:
-        assert P["segs"][P["leaf"][t]][5] == -1
-    for t in P["merge"].tolist():  # every piece that holds a merged token's rows is on its way to the root
-        chain, s = set(), int(P["leaf"][t])
+    joined = P["merge"].tolist()
+    assert [t for t, _, _ in joined] == sorted(inside)
+    for t, token, leaf in joined:  # every piece that holds a joined token's rows is on its way to the root
+        assert token == P["perm"][t]
+        chain, s = set(), leaf
         while s >= 0:
+            assert 0 <= t - segs[s][0] < segs[s][1] // group
             chain.add(s)
-            s = int(P["segs"][s][5])
-        for (kind, w), (s, _, _) in at_item.items():
-            it = P["tile" if kind else "few"][w].tolist()
-            inside = it[0] + it[1] // group <= t <= it[0] + (it[1] + it[2] - 1) // group
-            assert not inside or s in chain
+            s = segs[s][6]
+        assert inside[t] <= chain
 
 
 def tree(H, rng, depth, width, lo, hi):
@@ -351,8 +345,8 @@ def test_shared_prefix_is_one_segment(host):
     kids = H.fork([root] * 40).tolist()
     H.extend(kids, [5] * 40)
     P = H.plan(kids, [1] * 40, group=4, kv_heads=8)
-    top = [s for s in P["segs"].tolist() if s[5] == -1]
-    assert len(top) == 1 and top[0][4] >= 128 and len(P["segs"]) == 41
+    top = [s for s in P["segs"].tolist() if s[6] == -1]
+    assert len(top) == 1 and top[0][5] >= 128 and len(P["segs"]) == 41
     keys = {(it[3], it[4]) for it in P["tile"].tolist()}
     assert min(k[0] for k in keys) == 0 and max(k[1] for k in keys) == 2048
     # a token inside the shared pages keeps its own causal limit: nothing behind it is shared
