@@ -198,6 +198,7 @@ class ShieldContext:
     def __init__(self, device_mask: int = 1):
         self._h = C.c_void_p()
         self._page_tokens = {}  # of each paged cache
+        self._most_pages = 64  # of a sequence, as far as kv_pages has seen
         _check(lib().shield_open(device_mask, C.byref(self._h)))
 
     def close(self):
@@ -394,10 +395,14 @@ class ShieldContext:
     def kv_pages(self, kv: int, seqs) -> np.ndarray:
         """The sequences' page numbers, one row each, padded with -1."""
         s = np.ascontiguousarray(seqs, np.int64)
-        most = -(-int(self.kv_lengths(kv, s).max(initial=0)) // self._page_tokens.get(kv, 1))
-        out = np.empty((s.size, most), np.int32)
-        _check(lib().shield_kv_pages(self._h, kv, _addr(s), s.size, None, _addr(out), most))
-        return out
+        lens = np.empty(s.size, np.int32)
+        out = np.empty((s.size, self._most_pages), np.int32)
+        rc = lib().shield_kv_pages(self._h, kv, _addr(s), s.size, _addr(lens), _addr(out), self._most_pages)
+        if rc == ERR_RANGE:  # room for longer lists than any so far
+            self._most_pages = int(self.kv_lengths(kv, s).max()) // 16 + 1
+            return self.kv_pages(kv, s)
+        _check(rc)
+        return out[:, :-(-int(lens.max(initial=0)) // self._page_tokens[kv])].copy()
 
     def kv_batch_create(self, kv: int, n_heads: int, max_tokens: int, max_seqs: int, max_positions: int) -> int:
         c = ShieldKvBatchConfig(n_heads, max_tokens, max_seqs, max_positions)

@@ -188,7 +188,7 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     SHIELD_CUDA(cudaMalloc(&B->part_ml, (size_t)S.max_part * sizeof(float2)));
     SHIELD_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&B->err), 4, cudaHostAllocMapped));
     *B->err = 0;
-    SHIELD_CUDA(cudaMemset(B->dev, 0, 16));  // no work until a plan is set
+    SHIELD_CUDA(cudaMemset(B->dev, 0, COUNTS * 4));  // no work until a plan is set
     auto ints = [&](size_t o) { return reinterpret_cast<const int32_t *>(B->dev + o); };
     DevPlan &P = B->plan;
     P.counts = ints(o_counts);
@@ -255,7 +255,7 @@ static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const
         memcpy(h + o, src, bytes);
         SHIELD_CUDA(cudaMemcpyAsync(B.dev + o, h + o, bytes, cudaMemcpyHostToDevice, s));
     };
-    const int32_t count[COUNTS] = {(int32_t)tokens, (int32_t)plan.few.size(), (int32_t)plan.tile.size(), (int32_t)plan.merge.size()};
+    const int32_t count[COUNTS] = {(int32_t)tokens, (int32_t)plan.few.size(), (int32_t)plan.tile.size(), (int32_t)plan.merge.size(), plan.solo};
     const DevPlan &P = B.plan;
     send(P.counts, count, sizeof(count));
     send(P.few, plan.few.data(), plan.few.size() * sizeof(Item));
@@ -349,11 +349,12 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     A.err = B.err;
     // A captured launch replays whatever plan is set then: enough CTAs for any,
     // each striding over the plan's own count.
-    const int64_t few = cap ? 2 * (int64_t)c.dev.sms : (int64_t)B.last.few.size() * c.pool.kv_heads;
+    const int64_t alone = (int64_t)B.last.solo * c.pool.kv_heads;
+    const int64_t few = cap ? 2 * (int64_t)c.dev.sms : (int64_t)B.last.few.size() * c.pool.kv_heads - alone + (alone + 3) / 4;
     const int64_t tile = cap ? (int64_t)c.dev.sms : (int64_t)B.last.tile.size() * c.pool.kv_heads;
     const int64_t join = cap ? std::min<int64_t>(B.max_tokens, 4096) : (int64_t)B.last.merge.size();
     check(launch_attend_tile(A, c.maps, tile, c.dev.sms, s), "attention, many rows");
-    check(launch_attend_few(A, few, s), "attention, few rows");
+    check(launch_attend_few(A, few, tile > 0, s), "attention, few rows");
     check(launch_attend_merge(A, join, s), "attention, joining");
 }
 

@@ -36,7 +36,11 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool valid
 // a run of keys: bound by reading the keys and values once. Four warps take
 // every fourth tile of 16 keys each, with a running (m, sum, o) of their own
 // and their own ring of cp.async stages, so no warp waits for another until
-// the four are joined at the end.
+// the four are joined at the end. Where the plan has more short pieces (up to
+// FEW_SOLO keys) than the GPU holds CTAs, a warp takes one alone: such a piece
+// is a chain of lookups and loads whose latency, not whose work, fills its
+// time, and four times as many are on their way (128 rows of 16 keys on
+// average: 20.9 -> 9.7 us).
 template <int D>
 struct FewShape {
     static constexpr int WARPS = 4;
@@ -58,14 +62,21 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
     __shared__ int dirty;
     const DevPool &P = A.pool;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t units = (int64_t)A.plan.counts[COUNT_FEW] * P.kv_heads;
-    const uint32_t ring = smem_addr(few_smem) + warp * S::STAGES * S::STAGE_BYTES;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    const int alone = A.plan.counts[COUNT_SOLO] * P.kv_heads;  // the last units of the list
+    const int shared = A.plan.counts[COUNT_FEW] * P.kv_heads - alone;
+    uint8_t *const own_smem = few_smem + warp * S::STAGES * S::STAGE_BYTES;
+    const uint32_t ring = smem_addr(own_smem);
+    for (int task = blockIdx.x; task < shared + (alone + S::WARPS - 1) / S::WARPS; task += gridDim.x) {
+        const bool solo = task >= shared;
+        const int u = solo ? shared + (task - shared) * S::WARPS + warp : task;
+        if (solo && u >= shared + alone) continue;  // nothing below is waited for by other warps
+        const int first = solo ? 0 : warp, step = solo ? 1 : S::WARPS;  // this warp's tiles
         const Item it = A.plan.few[u / P.kv_heads];
-        const int kvh = (int)(u % P.kv_heads);
+        const int kvh = u % P.kv_heads;
         const int32_t *table = A.plan.table + it.table;
         const int ntiles = (it.k1 - it.k0 + S::KEYS - 1) / S::KEYS;
-        if (threadIdx.x == 0) dirty = 0;
+        if (threadIdx.x == 0 && !solo) dirty = 0;
 
         auto load = [&](int t, int stage) {
             const int p0 = it.k0 + t * S::KEYS;
@@ -83,7 +94,7 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
         };
 #pragma unroll
         for (int s = 0; s < S::STAGES - 1; s++) {
-            if (warp + s * S::WARPS < ntiles) load(warp + s * S::WARPS, s);
+            if (first + s * step < ntiles) load(first + s * step, s);
             asm volatile("cp.async.commit_group;" ::: "memory");
         }
 
@@ -115,7 +126,7 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
         bool found = false;
 
         int stage = 0;
-        for (int t = warp; t < ntiles; t += S::WARPS) {
+        for (int t = first; t < ntiles; t += step) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::STAGES - 2) : "memory");
             __syncwarp();
             const uint32_t ks = ring + stage * S::STAGE_BYTES, vs = ks + S::TILE_BYTES;
@@ -186,7 +197,7 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                 H::mma(o[2 * np + 1], pf, b[2], b[3]);
             }
             __syncwarp();
-            const int ahead = t + (S::STAGES - 1) * S::WARPS;
+            const int ahead = t + (S::STAGES - 1) * step;
             if (ahead < ntiles) load(ahead, stage == 0 ? S::STAGES - 1 : stage - 1);
             asm volatile("cp.async.commit_group;" ::: "memory");
             stage = stage + 1 == S::STAGES ? 0 : stage + 1;
@@ -196,6 +207,51 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
         for (int e = 0; e < 2; e++) {
             sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 1);
             sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
+        }
+        // Writes four dims of a row, which the warps' outputs add up to.
+        auto put = [&](int r, int d, float4 x, float M, float L, bool fix) {
+            const int at = it.tok0 + (it.r0 + r) / A.group, head = kvh * A.group + (it.r0 + r) % A.group;
+            if (fix) {
+                const int end = min(it.k1, A.plan.lim[at]);
+                for (int p = it.k0 + (max(low - it.k0, 0) / S::KEYS) * S::KEYS; p < end; p++) {
+                    const uint16_t *v = static_cast<const uint16_t *>(P.v) +
+                        row_offset(P, A.layer, table[p >> P.page_shift], kvh, p & (P.page_tokens - 1)) + d;
+                    if ((v[0] & H::EXP) == H::EXP) x.x += H::value(v[0]);
+                    if ((v[1] & H::EXP) == H::EXP) x.y += H::value(v[1]);
+                    if ((v[2] & H::EXP) == H::EXP) x.z += H::value(v[2]);
+                    if ((v[3] & H::EXP) == H::EXP) x.w += H::value(v[3]);
+                }
+            }
+            if (it.part < 0) {
+                const float inv = 1.0f / L;
+                uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + d;
+                *reinterpret_cast<uint2 *>(out) = make_uint2(H::pack(x.x * inv, x.y * inv), H::pack(x.z * inv, x.w * inv));
+            } else {
+                const int64_t part = it.part + (int64_t)kvh * it.nr + r;
+                *reinterpret_cast<float4 *>(A.plan.part_o + part * D + d) = x;
+                if (d == 0) A.plan.part_ml[part] = make_float2(M, L);
+            }
+        };
+        if (solo) {
+            const bool fix = __any_sync(0xffffffffu, found);
+            float *join = reinterpret_cast<float *>(own_smem);  // this warp's ring is free
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int r = (lane >> 2) + 8 * e;
+                if ((lane & 3) == 0) join_ml[warp][r] = make_float2(m[e], sum[e]);
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+                    *reinterpret_cast<float2 *>(join + r * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+            }
+            __syncwarp();
+            for (int i = lane; i < it.nr * (D / 4); i += 32) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                const float2 ml = join_ml[warp][r];
+                put(r, d, *reinterpret_cast<const float4 *>(join + r * D + d), ml.x, ml.y, fix);
+            }
+            __syncwarp();  // the ring is free for the next unit
+            continue;
         }
         __syncthreads();  // every warp is done with its ring; dirty is set to 0
         float *join = reinterpret_cast<float *>(few_smem);
@@ -221,9 +277,6 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                 w[i] = exp2_approx(join_ml[i][r].x - (M == -INFINITY ? 0.0f : M));
                 L = __fmaf_rn(join_ml[i][r].y, w[i], L);
             }
-            const int at = it.tok0 + (it.r0 + r) / A.group, head = kvh * A.group + (it.r0 + r) % A.group;
-            const int64_t part = it.part + (int64_t)kvh * it.nr + r;
-            const float inv = it.part < 0 ? 1.0f / L : 1.0f;
 #pragma unroll
             for (int j = 0; j < D / 32; j++) {
                 const int d = j * 32 + (threadIdx.x & 7) * 4;
@@ -236,44 +289,28 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                     a.z = __fmaf_rn(x.z, w[i], a.z);
                     a.w = __fmaf_rn(x.w, w[i], a.w);
                 }
-                if (dirty) {
-                    const int end = min(it.k1, A.plan.lim[at]);
-                    for (int p = it.k0 + (max(low - it.k0, 0) / S::KEYS) * S::KEYS; p < end; p++) {
-                        const uint16_t *v = static_cast<const uint16_t *>(P.v) +
-                            row_offset(P, A.layer, table[p >> P.page_shift], kvh, p & (P.page_tokens - 1)) + d;
-                        if ((v[0] & H::EXP) == H::EXP) a.x += H::value(v[0]);
-                        if ((v[1] & H::EXP) == H::EXP) a.y += H::value(v[1]);
-                        if ((v[2] & H::EXP) == H::EXP) a.z += H::value(v[2]);
-                        if ((v[3] & H::EXP) == H::EXP) a.w += H::value(v[3]);
-                    }
-                }
-                if (it.part < 0) {
-                    uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + d;
-                    *reinterpret_cast<uint2 *>(out) = make_uint2(H::pack(a.x * inv, a.y * inv), H::pack(a.z * inv, a.w * inv));
-                } else {
-                    *reinterpret_cast<float4 *>(A.plan.part_o + part * D + d) = a;
-                    if ((threadIdx.x & 7) == 0 && j == 0) A.plan.part_ml[part] = make_float2(M, L);
-                }
+                put(r, d, a, M, L, dirty != 0);
             }
         }
         __syncthreads();  // the ring and join_ml are free for the next unit
     }
+    // (launched while the many-row kernel still runs: this one is not over before that is)
+    if (blockIdx.x == gridDim.x - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 template <bool BF16, int D>
-static cudaError_t few_launch(const AttendArgs &A, int64_t units, cudaStream_t s) {
+static cudaError_t few_launch(const AttendArgs &A, int64_t units, bool beside, cudaStream_t s) {
     using S = FewShape<D>;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(k_attend_few<BF16, D>, S::BYTES, allowed);
     if (e != cudaSuccess) return e;
-    k_attend_few<BF16, D><<<(unsigned)std::min<int64_t>(units, 1 << 30), 128, S::BYTES, s>>>(A);
-    return cudaGetLastError();
+    return launch_early(k_attend_few<BF16, D>, (unsigned)units, 128, S::BYTES, beside, s, A);
 }
 
-cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s) {
+cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, bool beside, cudaStream_t s) {
     if (units == 0) return cudaSuccess;
-    if (A.pool.dim == 128) return A.pool.bf16 ? few_launch<true, 128>(A, units, s) : few_launch<false, 128>(A, units, s);
-    if (A.pool.dim == 64) return A.pool.bf16 ? few_launch<true, 64>(A, units, s) : few_launch<false, 64>(A, units, s);
+    if (A.pool.dim == 128) return A.pool.bf16 ? few_launch<true, 128>(A, units, beside, s) : few_launch<false, 128>(A, units, beside, s);
+    if (A.pool.dim == 64) return A.pool.bf16 ? few_launch<true, 64>(A, units, beside, s) : few_launch<false, 64>(A, units, beside, s);
     return cudaErrorInvalidValue;
 }
 
@@ -289,6 +326,7 @@ __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
     constexpr int E = D / 32;
     const int lane = threadIdx.x & 31;
     const int heads = A.group * A.pool.kv_heads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // launched early: the partials are there from here on
     const int64_t rows = (int64_t)A.plan.counts[COUNT_MERGE] * heads;
     for (int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); w < rows; w += (int64_t)gridDim.x * 4) {
         const Join J = A.plan.merge[w / heads];
@@ -351,8 +389,7 @@ __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
 template <bool BF16, int D>
 static cudaError_t merge_launch(const AttendArgs &A, int64_t tokens, cudaStream_t s) {
     const int64_t rows = tokens * A.group * A.pool.kv_heads;
-    k_attend_merge<BF16, D><<<(unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 30), 128, 0, s>>>(A);
-    return cudaGetLastError();
+    return launch_early(k_attend_merge<BF16, D>, (unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 30), 128, 0, true, s, A);
 }
 
 cudaError_t launch_attend_merge(const AttendArgs &A, int64_t tokens, cudaStream_t s) {

@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     volatile int *const dirty = reinterpret_cast<volatile int *>(smem + S::OFF_MISC + 8);
     float2 *const join_ml = reinterpret_cast<float2 *>(smem + S::OFF_JOIN);
 
+    asm volatile("griddepcontrol.launch_dependents;");
     if (threadIdx.x == 0) {
         for (int a = 0; a < 2; a++) {
             for (int h = 0; h < 2; h++) {

@@ -33,9 +33,20 @@ __global__ void __launch_bounds__(256) k_move_pages(const __grid_constant__ Move
     char *dst = base + mv.dst * page_bytes;
     const int vecs = mv.rows * pool.dim / 8;  // 16-byte vectors of one head's rows
     const int total = vecs * pool.kv_heads;
-    for (int i = threadIdx.x; i < total; i += blockDim.x) {
-        const int64_t off = (int64_t)(i / vecs) * head_bytes + (int64_t)(i % vecs) * 16;
-        *reinterpret_cast<uint4 *>(dst + off) = *reinterpret_cast<const uint4 *>(src + off);
+    // eight vectors of a thread are on their way together
+    for (int i0 = threadIdx.x; i0 < total; i0 += 8 * 256) {
+        uint4 x[8];
+        int64_t off[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int i = i0 + j * 256;
+            if (i >= total) break;
+            off[j] = (int64_t)(i / vecs) * head_bytes + (int64_t)(i % vecs) * 16;
+            x[j] = *reinterpret_cast<const uint4 *>(src + off[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (i0 + j * 256 < total) *reinterpret_cast<uint4 *>(dst + off[j]) = x[j];
     }
 }
 
@@ -67,7 +78,7 @@ __device__ __forceinline__ uint32_t pack_pair(float a, float b, bool bf16) {
     return *reinterpret_cast<const uint32_t *>(&r);
 }
 
-// One thread per 8 values of a row (one 16-byte store); f32 sources are
+// A thread moves 8 values of a row at a time (one 16-byte store); f32 sources are
 // rounded once, to nearest even. blockIdx.y: 0 keys, 1 values.
 template <bool F32>
 __global__ void __launch_bounds__(256) k_write_rows(const DevPool pool, const DevPlan plan, int layer, const void *k,
@@ -78,21 +89,32 @@ __global__ void __launch_bounds__(256) k_write_rows(const DevPool pool, const De
     const int64_t stride = blockIdx.y ? v_stride : k_stride;
     uint16_t *dst = static_cast<uint16_t *>(blockIdx.y ? pool.v : pool.k) + (int64_t)layer * pool.layer_stride();
     const int per_head = pool.dim / 8;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t t = i / per_tok;
-        const int c = (int)(i - t * per_tok), h = c / per_head, d = (c - h * per_head) * 8;
-        const int slot = plan.slot[t];
-        const int64_t page = slot >> pool.page_shift, row = slot & (pool.page_tokens - 1);
-        uint4 o;
-        if (F32) {
-            const float4 *p = reinterpret_cast<const float4 *>(src + (t * stride + c * 8) * 4);
-            const float4 a = p[0], b = p[1];
-            o = make_uint4(pack_pair(a.x, a.y, pool.bf16), pack_pair(a.z, a.w, pool.bf16),
-                           pack_pair(b.x, b.y, pool.bf16), pack_pair(b.z, b.w, pool.bf16));
-        } else {
-            o = *reinterpret_cast<const uint4 *>(src + (t * stride + c * 8) * 2);
+    // four vectors of a thread are on their way together
+    constexpr int AT_ONCE = 4;
+    for (int64_t i0 = (int64_t)blockIdx.x * (256 * AT_ONCE) + threadIdx.x; i0 < n; i0 += (int64_t)gridDim.x * (256 * AT_ONCE)) {
+        uint4 o[AT_ONCE];
+        int64_t to[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            const int64_t i = i0 + j * 256;
+            if (i >= n) break;
+            const int64_t t = i / per_tok;
+            const int c = (int)(i - t * per_tok), h = c / per_head, d = (c - h * per_head) * 8;
+            const int slot = plan.slot[t];
+            const int64_t page = slot >> pool.page_shift, row = slot & (pool.page_tokens - 1);
+            to[j] = (((page * pool.kv_heads + h) << pool.page_shift) + row) * pool.dim + d;
+            if (F32) {
+                const float4 *p = reinterpret_cast<const float4 *>(src + (t * stride + c * 8) * 4);
+                const float4 a = p[0], b = p[1];
+                o[j] = make_uint4(pack_pair(a.x, a.y, pool.bf16), pack_pair(a.z, a.w, pool.bf16),
+                                  pack_pair(b.x, b.y, pool.bf16), pack_pair(b.z, b.w, pool.bf16));
+            } else {
+                o[j] = *reinterpret_cast<const uint4 *>(src + (t * stride + c * 8) * 2);
+            }
         }
-        *reinterpret_cast<uint4 *>(dst + (((page * pool.kv_heads + h) << pool.page_shift) + row) * pool.dim + d) = o;
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++)
+            if (i0 + j * 256 < n) *reinterpret_cast<uint4 *>(dst + to[j]) = o[j];
     }
 }
 
@@ -100,7 +122,7 @@ cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t 
                               const void *k, int64_t k_stride, const void *v, int64_t v_stride, cudaStream_t s) {
     const int64_t n = tokens * pool.kv_heads * pool.dim / 8;
     if (n == 0) return cudaSuccess;
-    const dim3 grid((unsigned)std::min<int64_t>((n + 255) / 256, 1 << 20), 2);
+    const dim3 grid((unsigned)std::min<int64_t>((n + 1023) / 1024, 1 << 20), 2);
     if (f32) k_write_rows<true><<<grid, 256, 0, s>>>(pool, plan, layer, k, k_stride, v, v_stride);
     else k_write_rows<false><<<grid, 256, 0, s>>>(pool, plan, layer, k, k_stride, v, v_stride);
     return cudaGetLastError();

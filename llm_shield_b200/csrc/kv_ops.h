@@ -24,7 +24,7 @@ struct DevPool {
 // batch's capacities and the counts live beside them, so a captured launch
 // reads whatever plan was uploaded last.
 struct DevPlan {
-    const int32_t *counts = nullptr;  // tokens, few items, tile items, tokens to join
+    const int32_t *counts = nullptr;  // tokens, few items, tile items, tokens to join, few items for a warp alone
     const int32_t *slot = nullptr, *perm = nullptr, *lim = nullptr, *where = nullptr, *table = nullptr;
     const Join *merge = nullptr;
     const Segment *segs = nullptr;
@@ -32,7 +32,7 @@ struct DevPlan {
     float *part_o = nullptr;   // [partial row][dim], not divided by the row's sum
     float2 *part_ml = nullptr; // running maximum (base-2 exponent) and sum of each partial row
 };
-enum { COUNT_TOKENS = 0, COUNT_FEW = 1, COUNT_TILE = 2, COUNT_MERGE = 3, COUNTS = 4 };
+enum { COUNT_TOKENS = 0, COUNT_FEW = 1, COUNT_TILE = 2, COUNT_MERGE = 3, COUNT_SOLO = 4, COUNTS = 5 };
 
 struct AttendArgs {
     DevPool pool;
@@ -52,9 +52,10 @@ cudaError_t launch_move_pages(const DevPool &pool, const Move *moves, int64_t n,
 // upper bound of later plans' (the kernel stops at the plan's count).
 cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t tokens, int32_t layer, bool f32,
                               const void *k, int64_t k_stride, const void *v, int64_t v_stride, cudaStream_t s);
-// The three attention kernels over `units` work units (or as many as a later
-// plan may have: each strides over the plan's own count).
-cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, cudaStream_t s);
+// The three attention kernels over `units` work units (or CTAs for as many as a
+// later plan may have: each strides over the plan's own count).
+// beside: launch_attend_tile came just before, and this one may run beside it.
+cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, bool beside, cudaStream_t s);
 // maps: map_pool of the keys and of the values, made once per pool.
 bool map_pool(CUtensorMap *m, const DevPool &pool, void *data);
 cudaError_t launch_attend_tile(const AttendArgs &A, const CUtensorMap *maps, int64_t units, int sms, cudaStream_t s);  // one persistent CTA per SM

@@ -254,14 +254,17 @@ struct Plan {
     std::vector<Join> merge;
     std::vector<int32_t> table;
     int64_t part_rows = 0;
+    int32_t solo = 0;                      // the last items of few, which a warp takes alone
     void clear() {
         slot.clear(); perm.clear(); lim.clear(); segs.clear(); few.clear(); tile.clear(); where.clear(); merge.clear();
         table.clear();
         part_rows = 0;
+        solo = 0;
     }
 };
 
 constexpr int32_t FEW_TILE = 16;  // rows of a few-row item
+constexpr int32_t FEW_SOLO = 64;  // keys that one warp may take alone
 constexpr int32_t KEY_STEP = 128; // splits are whole steps of this many keys
 
 namespace detail {
@@ -464,7 +467,7 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
                     P.part_rows += (int64_t)it.nr * S.kv_heads;
                     if (P.part_rows > S.max_part) return false;
                 }
-                const int64_t cost = (int64_t)((it.k1 - it.k0 + KEY_STEP - 1) / KEY_STEP) * (it.nr > 128 ? 2 : 1);
+                const int64_t cost = (int64_t)(it.k1 - it.k0) * (it.nr > 128 ? 2 : 1);
                 refs.push_back({cost, it, few});
                 P.where.push_back(it.part);
             }
@@ -473,6 +476,9 @@ inline bool make_plan_with(const Pool &pool, const int64_t *ids, const int32_t *
     if ((int64_t)P.segs.size() > S.max_segments) return false;
     std::stable_sort(refs.begin(), refs.end(), [](const Ref &a, const Ref &b) { return a.cost > b.cost; });
     for (const Ref &r : refs) (r.few ? P.few : P.tile).push_back(r.it);
+    // short pieces go to single warps when there are more than CTAs side by side
+    if ((int64_t)P.few.size() * S.kv_heads > 2 * (int64_t)S.sms)
+        for (const Item &it : P.few) P.solo += it.k1 - it.k0 <= FEW_SOLO;
     for (int32_t t = 0; t < (int32_t)P.perm.size(); t++)
         if (!P.segs[leaf[t]].direct) P.merge.push_back({t, P.perm[t], leaf[t]});
     return true;

@@ -267,9 +267,9 @@ def check_plan(H, ids, counts, P, group, kv_heads):
             tok0, r0, nr, k0, k1, table, part, masked = it
             assert 1 <= nr <= (FEW_TILE if kind == 0 else 256)
             assert 0 <= k0 < k1 and k0 % pt == 0
-            blocks = -(-(k1 - k0) // 128) * (2 if nr > 128 else 1)
-            assert cost is None or blocks <= cost  # longest first
-            cost = blocks
+            keys = (k1 - k0) * (2 if nr > 128 else 1)
+            assert cost is None or keys <= cost  # longest first
+            cost = keys
             if part >= 0:
                 s, sp, t = of_part.pop(part)
                 assert segs[s][0] == tok0 and r0 == t * segs[s][5] and nr == min(segs[s][5], segs[s][1] - r0)
