@@ -59,7 +59,8 @@ struct DeviceScope {
     int before = -1;
     explicit DeviceScope(int ordinal) {
         if (cudaGetDevice(&before) != cudaSuccess) before = -1;
-        SHIELD_CUDA(cudaSetDevice(ordinal));
+        if (before == ordinal) before = -1;
+        else SHIELD_CUDA(cudaSetDevice(ordinal));
     }
     ~DeviceScope() {
         if (before >= 0) cudaSetDevice(before);

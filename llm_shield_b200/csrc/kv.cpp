@@ -347,6 +347,11 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     A.group = B.shape.group;
     A.scale_log2 = scale * 1.44269504088896340736f;
     A.err = B.err;
+    if (!cap) {
+        A.few = (int32_t)B.last.few.size();
+        A.solo = B.last.solo;
+        A.tile = (int32_t)B.last.tile.size();
+    }
     // A captured launch replays whatever plan is set then: enough CTAs for any,
     // each striding over the plan's own count.
     const int64_t alone = (int64_t)B.last.solo * c.pool.kv_heads;

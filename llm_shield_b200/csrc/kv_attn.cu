@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
     const DevPool &P = A.pool;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;");
-    const int alone = A.plan.counts[COUNT_SOLO] * P.kv_heads;  // the last units of the list
-    const int shared = A.plan.counts[COUNT_FEW] * P.kv_heads - alone;
+    const int alone = (A.solo >= 0 ? A.solo : A.plan.counts[COUNT_SOLO]) * P.kv_heads;  // the last units of the list
+    const int shared = (A.few >= 0 ? A.few : A.plan.counts[COUNT_FEW]) * P.kv_heads - alone;
     uint8_t *const own_smem = few_smem + warp * S::STAGES * S::STAGE_BYTES;
     const uint32_t ring = smem_addr(own_smem);
     for (int task = blockIdx.x; task < shared + (alone + S::WARPS - 1) / S::WARPS; task += gridDim.x) {

@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a's half h at 128 a + 64 h, O at 256 + 128 a
 
-    const int units = A.plan.counts[COUNT_TILE] * P.kv_heads;  // the host keeps it, and one more round, below 2^31
+    const int units = (A.tile >= 0 ? A.tile : A.plan.counts[COUNT_TILE]) * P.kv_heads;  // the host keeps it, and one more round, below 2^31
     // A barrier only tells the parity of its phase, so whoever waits on one waits
     // for each of its phases in turn, and none can pass before all who wait have
     // seen it: every ring slot is released by both tiles, whoever uses it.
@@ -475,6 +475,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
         const float scale = fmaxf(fabsf(A.scale_log2), 1e-30f);  // a zero scale still keeps masked scores at -inf
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t st = tmem + lanes + 128 * a, ot = tmem + lanes + 256 + 128 * a;
+        const uint32_t join_row = base + row * D * 4;  // 16-byte chunks xor-ed with the row against bank conflicts
         uint32_t ring = 0, turn = 0;
         uint32_t done = 0;          // key blocks of this tile in earlier units
         uint32_t ends = 0;          // earlier units in which this tile had a block
@@ -612,7 +613,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             if (two) {
                 if (a == 1) {
                     // no product reads the queries any more once tile 0 is done too:
-                    // their place takes this tile's outputs, [dim][row]
+                    // their place takes this tile's outputs, a row a thread
                     if (ok) ok = mbar_wait_warp_timed(join_ready, joins & 1, stop, A.err);
                     if (ok && live) {
                         tc_fence_after();
@@ -621,7 +622,9 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                             uint32_t o[32];
                             tmem_load32_wait(ot + c, o);
 #pragma unroll
-                            for (int i = 0; i < 32; i++) *reinterpret_cast<uint32_t *>(smem + ((c + i) * ROWS + row) * 4) = o[i];
+                            for (int i = 0; i < 32; i += 4)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(join_row + (((c + i) / 4 ^ (row & 7)) << 4)),
+                                             "r"(o[i]), "r"(o[i + 1]), "r"(o[i + 2]), "r"(o[i + 3]) : "memory");
                         }
                     }
                     join_ml[row] = make_float2(m, sum);
@@ -669,9 +672,12 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     tmem_load32_wait(ot + c, o);
                     if (two) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) {
-                            const float y = *reinterpret_cast<const float *>(smem + ((c + j) * ROWS + row) * 4);
-                            o[j] = __float_as_uint(__fmaf_rn(y, f1, __uint_as_float(o[j]) * f0));
+                        for (int j = 0; j < 32; j += 4) {
+                            float y[4];
+                            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3])
+                                         : "r"(join_row + (((c + j) / 4 ^ (row & 7)) << 4)) : "memory");
+#pragma unroll
+                            for (int k = 0; k < 4; k++) o[j + k] = __float_as_uint(__fmaf_rn(y[k], f1, __uint_as_float(o[j + k]) * f0));
                         }
                     }
                     if (fix && mine) {

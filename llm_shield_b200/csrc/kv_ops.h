@@ -41,6 +41,7 @@ struct AttendArgs {
     void *out = nullptr;
     int64_t q_stride = 0, out_stride = 0;  // elements from token to token
     int32_t layer = 0, group = 1;
+    int32_t few = -1, solo = -1, tile = -1;  // the plan's counts where the host knows them: one lookup less
     float scale_log2 = 0.0f;               // scale * log2(e)
     int32_t *err = nullptr;                // error word of bounded waits
 };
