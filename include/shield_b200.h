@@ -337,6 +337,23 @@ shield_status shield_kv_attend(shield_ctx *ctx, int64_t batch, int32_t layer, co
                                int64_t out_stride, float scale, void *stream);
 
 /*
+ * shield_seq_forward on sequences of a paged cache of the configured model's
+ * shape (n_layers, n_kv_heads, head_dim): appends ids[offsets[i] ..
+ * offsets[i+1]) to sequence seqs[i] (each once per call), in batches of up to
+ * max_batch_tokens on the context's stream of the cache's GPU, and writes each
+ * sequence's whole tied head at its new last position to logits[i * vocab ..]
+ * when logits is non-null. Keys and values are the exact path's, rounded to
+ * the cache's type; the attention is shield_kv_attend's, on queries rounded
+ * to that type, so logits differ from the exact path's in their last digits
+ * and follow the batch's plan. Everything else is bit-identical to it. If the
+ * call fails, no sequence has changed. SHIELD_ERR_RANGE beyond max_positions,
+ * SHIELD_ERR_NOMEM when the pool has too few pages. The cache's contents are
+ * its user's: they are kept when weights are uploaded again.
+ */
+shield_status shield_kv_forward(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *ids,
+                                const int64_t *offsets, int32_t n, float *logits, const volatile int32_t *cancel);
+
+/*
  * QuantMatMul.ForwardAsync / ForwardRowsAsync (Numerics/QuantMatMul.cs:71-110)
  * on one GPU of the context, host buffers in and out:
  *   y[t, i] = dot(x[t, :], W[row(i), :]),  x: M x cols, y: M x n_out

@@ -82,6 +82,7 @@ EXPORTS = [
     "shield_kv_create", "shield_kv_release", "shield_kv_get_info", "shield_kv_open", "shield_kv_extend",
     "shield_kv_fork", "shield_kv_copy", "shield_kv_free", "shield_kv_compact", "shield_kv_pages",
     "shield_kv_batch_create", "shield_kv_batch_release", "shield_kv_batch_set", "shield_kv_write", "shield_kv_attend",
+    "shield_kv_forward",
 ]
 
 _lib = None
@@ -140,6 +141,7 @@ def lib() -> C.CDLL:
         L.shield_kv_batch_set.argtypes = [P, I64, P, P, I32, P]
         L.shield_kv_write.argtypes = [P, I64, I32, C.c_uint32, P, I64, P, I64, P]
         L.shield_kv_attend.argtypes = [P, I64, I32, P, I64, P, I64, C.c_float, P]
+        L.shield_kv_forward.argtypes = [P, I64, P, P, P, I32, P, P]
         L.shield_last_error.restype = C.c_char_p
         for name in EXPORTS:
             f = getattr(L, name)
@@ -429,6 +431,19 @@ class ShieldContext:
                   stream: int | None = None) -> None:
         """The step's causal attention in one layer."""
         _check(lib().shield_kv_attend(self._h, batch, layer, q, q_stride, out, out_stride, scale, _kv_stream(stream)))
+
+    def kv_forward(self, kv: int, seqs, chunks, want_logits: bool = True, cancel: np.ndarray | None = None):
+        """Appends chunks[i] (int32 ids) to paged sequence seqs[i] through the
+        model; returns the (n, vocab) logits at each one's new last position."""
+        s = np.ascontiguousarray(seqs, np.int64)
+        if s.size != len(chunks):
+            raise ValueError("one chunk per sequence")
+        ids, offsets = self._pack(chunks)
+        out = np.zeros((len(chunks), self.spec.vocab), np.float32) if want_logits else None
+        _check(lib().shield_kv_forward(self._h, kv, _addr(s), _addr(ids), _addr(offsets), len(chunks),
+                                       _addr(out) if out is not None else None,
+                                       _p(cancel) if cancel is not None else None))
+        return out
 
     def qmatmul(self, weight: str, x: np.ndarray, M: int, n_out: int, row_ids=None, device: int = 0):
         x = np.ascontiguousarray(x, np.float32)

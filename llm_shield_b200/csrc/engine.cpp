@@ -505,9 +505,12 @@ struct Batch {  // one micro-batch of whole requests on one device
 // d.buf.h_logits after a stream sync. full_logits (host, R x vocab): the whole
 // tied head at every last position instead. store_prefix: the batch is the
 // prefix alone; its per-layer keys and values are kept in d.pre_k / d.pre_v.
+// paged: a planned step of a paged cache, whose keys, values and attention are
+// that cache's, in its 16-bit type (the exact attention's work list is unused).
 static void forward_batch(Ctx &C, Device &d, const int32_t *ids_host, const Batch &B, int nv,
                           const volatile int32_t *cancel, int capture_layer, int capture_what, float *capture,
-                          float *full_logits = nullptr, bool store_prefix = false, bool graph = false) {
+                          float *full_logits = nullptr, bool store_prefix = false, bool graph = false,
+                          kv::Batch *paged = nullptr) {
     const Config &c = C.cfg;
     const int64_t M = B.tokens;
     const int R = (int)B.req.size();
@@ -730,8 +733,8 @@ static void forward_batch(Ctx &C, Device &d, const int32_t *ids_host, const Batc
         }
         count_launch(d), check_launch(launch_rope_qk(b.q, c.n_heads, b.k, c.n_kv_heads, M, c.head_dim, d_pos, d.cos_t,
                                                     d.sin_t, c.rope_half, d.temp, b.ctx, b.kc,
-                                                    l == capture_layer && capture_what == SHIELD_ACT_Q_ROPE,
-                                                    l == capture_layer && capture_what == SHIELD_ACT_K_ROPE, s),
+                                                    paged || (l == capture_layer && capture_what == SHIELD_ACT_Q_ROPE),
+                                                    paged || (l == capture_layer && capture_what == SHIELD_ACT_K_ROPE), s),
                                      "rope");
         cap(l, SHIELD_ACT_Q_ROPE, b.q, c.qdim());
         cap(l, SHIELD_ACT_K_ROPE, b.k, c.kvdim());
@@ -767,7 +770,18 @@ static void forward_batch(Ctx &C, Device &d, const int32_t *ids_host, const Batc
             a1 = T.event();
             if (a0) cudaEventRecord(a0, s);
         }
+        if (paged) {
+            // queries and outputs in the cache's type, in the scores' scratch
+            const bool bf16 = paged->cache->pool.bf16;
+            void *q16 = b.scores, *o16 = reinterpret_cast<uint16_t *>(b.scores) + M * c.qdim();
+            kv::write_layer(*paged, l, b.k, b.v, s);
+            check_launch(kv::launch_narrow(b.q, q16, M * c.qdim(), bf16, s), "round queries");
+            kv::attend_layer(*paged, l, q16, o16, scale, s);
+            check_launch(kv::launch_widen(o16, b.ctx, M * c.qdim(), bf16, s), "widen context");
+            d.timing.launches += 3 + !paged->last.few.empty() + !paged->last.tile.empty() + !paged->last.merge.empty();
+        }
         for (const AttGroup &ag : groups) {
+            if (paged) break;
             d.timing.launches += 1;
             A.work = d_work + ag.w0;
             A.work_base = d_wbase + ag.w0;
@@ -1485,6 +1499,69 @@ static void seq_forward(Ctx &C, const int64_t *seq, const int32_t *ids, const in
         if (codes[di] != SHIELD_OK) throw Error(codes[di], errors[di]);
 }
 
+// As seq_forward, on sequences of a paged cache of the model's shape.
+static void kv_forward(shield_ctx *handle, Ctx &C, int64_t kv_id, const int64_t *seq, const int32_t *ids, const int64_t *offsets,
+                       int32_t n, float *logits, const volatile int32_t *cancel) {
+    if (!C.configured) throw Error(SHIELD_ERR_STATE, "no model configured");
+    kv::Cache &K = kv::cache_of(handle, kv_id);
+    if (n < 0 || (n > 0 && (!seq || !ids || !offsets))) throw Error(SHIELD_ERR_ARG, "null buffer");
+    const Config &c = C.cfg;
+    if (K.pool.layers != c.n_layers || K.pool.kv_heads != c.n_kv_heads || K.pool.dim != c.head_dim)
+        throw Error(SHIELD_ERR_SHAPE, "the cache's layers, kv heads and head_dim are not the model's");
+    if (n == 0) return;
+    if (offsets[0] != 0) throw Error(SHIELD_ERR_ARG, "offsets[0] must be 0");
+    std::vector<int32_t> count(n), had(n);
+    int32_t longest = 0;
+    for (int32_t i = 0; i < n; i++) {
+        const kv::Sequence &sq = K.book.get(seq[i]);
+        const int64_t len = offsets[i + 1] - offsets[i];
+        if (len <= 0) throw Error(SHIELD_ERR_ARG, "sequence entry " + std::to_string(i) + " has no tokens");
+        if (sq.len + len > c.max_positions)
+            throw Error(SHIELD_ERR_RANGE, "sequence " + std::to_string(seq[i]) + " would hold " + std::to_string(sq.len + len) +
+                                              " positions, more than max_positions " + std::to_string(c.max_positions));
+        count[i] = (int32_t)len;
+        had[i] = sq.len;
+        longest = std::max(longest, sq.len + count[i]);
+    }
+    validate_ids(C, ids, offsets[n]);
+    Device &d = *C.devs[K.device];
+    DeviceScope scope(d.ordinal);
+    ensure_buffers(C, d);
+    if ((int64_t)c.max_batch_tokens * c.qdim() > d.buf.scores_cap)
+        throw Error(SHIELD_ERR_UNSUPPORTED, "max_batch_tokens is too large for a paged forward's scratch");
+    K.book.extend(seq, count.data(), n);
+    const int64_t V = c.vocab;
+    std::vector<int32_t> packed;
+    std::vector<float> full;
+    try {
+        for (int32_t k = 0; k < n;) {
+            Batch B;
+            const int32_t first = k;
+            while (k < n && (B.req.empty() || B.tokens + count[k] <= c.max_batch_tokens)) {
+                B.req.push_back(k);
+                B.start.push_back(B.tokens);
+                B.len.push_back(count[k]);
+                B.pre.push_back(had[k]);
+                // the exact attention's work list wants a cache for what comes before
+                B.ck.push_back(d.buf.kc);
+                B.cv.push_back(d.buf.v);
+                B.cstride.push_back(0);
+                B.append.push_back(0);
+                B.tokens += count[k++];
+            }
+            kv::Batch &step = kv::model_batch(K, c.n_heads, (int32_t)B.tokens, k - first, longest);
+            kv::set_batch(step, seq + first, count.data() + first, k - first, d.stream);
+            packed.assign(ids + offsets[first], ids + offsets[k]);
+            full.resize((size_t)(k - first) * V);
+            forward_batch(C, d, packed.data(), B, 0, cancel, -1, 0, nullptr, full.data(), false, false, &step);
+            if (logits) memcpy(logits + (int64_t)first * V, full.data(), full.size() * 4);
+        }
+    } catch (...) {
+        K.book.undo_extend(seq, count.data(), n);
+        throw;
+    }
+}
+
 static void seq_reset(Ctx &C, int64_t id) { sequence_of(C, id, nullptr).len = 0; }
 
 static void seq_release(Ctx &C, int64_t id) {
@@ -1646,6 +1723,14 @@ shield_status shield_seq_forward(shield_ctx *ctx, const int64_t *seqs, const int
     return guarded([&] {
         if (!ctx) throw Error(SHIELD_ERR_ARG, "ctx is null");
         seq_forward(ctx->c, seqs, ids, offsets, n, logits, cancel);
+    });
+}
+
+shield_status shield_kv_forward(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *ids,
+                                const int64_t *offsets, int32_t n, float *logits, const volatile int32_t *cancel) {
+    return guarded([&] {
+        if (!ctx) throw Error(SHIELD_ERR_ARG, "ctx is null");
+        kv_forward(ctx, ctx->c, kv, seqs, ids, offsets, n, logits, cancel);
     });
 }
 

@@ -10,6 +10,7 @@ namespace shield {
 namespace kv {
 
 Cache::~Cache() {
+    model.reset();
     if (!owns) return;
     int before = -1;
     cudaGetDevice(&before);
@@ -37,7 +38,7 @@ Batch::~Batch() {
     if (before >= 0) cudaSetDevice(before);
 }
 
-static Cache &cache_of(shield_ctx *ctx, int64_t id) {
+Cache &cache_of(shield_ctx *ctx, int64_t id) {
     if (!ctx) throw Error(SHIELD_ERR_ARG, "ctx is null");
     State &S = kv_state(ctx);
     auto it = S.caches.find(id);
@@ -99,6 +100,7 @@ static void create(shield_ctx *ctx, int32_t device, const shield_kv_config *cfg,
     auto cache = std::make_unique<Cache>(Pool(c.n_pages, c.page_tokens, (id << 32) + 1));
     cache->id = id;
     cache->dev = dev;
+    cache->device = device;
     DevPool &P = cache->pool;
     P.bf16 = c.type == SHIELD_TYPE_BF16;
     P.layers = c.n_layers;
@@ -142,9 +144,7 @@ static void fork(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t
     std::copy(ids.begin(), ids.end(), out);
 }
 
-static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_config *cfg, int64_t *out) {
-    Cache &c = cache_of(ctx, kv);
-    if (!cfg || !out) throw Error(SHIELD_ERR_ARG, "null argument");
+static std::unique_ptr<Batch> make_batch(Cache &c, const shield_kv_batch_config *cfg) {
     if (cfg->n_heads <= 0 || cfg->n_heads % c.pool.kv_heads)
         throw Error(SHIELD_ERR_SHAPE, std::to_string(cfg->n_heads) + " query heads do not divide into " +
                                           std::to_string(c.pool.kv_heads) + " kv heads");
@@ -203,9 +203,31 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     P.table = ints(o_table);
     P.part_o = B->part_o;
     P.part_ml = B->part_ml;
+    return B;
+}
+
+static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_config *cfg, int64_t *out) {
+    Cache &c = cache_of(ctx, kv);
+    if (!cfg || !out) throw Error(SHIELD_ERR_ARG, "null argument");
+    auto B = make_batch(c, cfg);
     State &st = kv_state(ctx);
     *out = st.next_batch++;
     st.batches.emplace(*out, std::move(B));
+}
+
+Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions) {
+    Batch *b = c.model.get();
+    if (b && b->n_heads == n_heads && b->max_tokens >= tokens && b->max_seqs >= seqs && b->max_positions >= positions) return *b;
+    shield_kv_batch_config cfg{n_heads, tokens, seqs, positions};
+    if (b && b->n_heads == n_heads) {
+        cfg.max_tokens = std::max(cfg.max_tokens, b->max_tokens);
+        cfg.max_seqs = std::max(cfg.max_seqs, b->max_seqs);
+        cfg.max_positions = std::max(cfg.max_positions, b->max_positions);
+    }
+    SHIELD_CUDA(cudaStreamSynchronize(c.dev.stream));
+    c.model.reset();
+    c.model = make_batch(c, &cfg);
+    return *c.model;
 }
 
 // The kernels' bounded waits report here; the host sees it at the next call.
@@ -216,12 +238,9 @@ static void check_error(Batch &B) {
     throw Error(SHIELD_ERR_TIMEOUT, "a device-side wait of an earlier call gave up (error word " + std::to_string(e) + ")");
 }
 
-static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const int32_t *counts, int32_t n, void *stream) {
-    Batch &B = batch_of(ctx, batch);
+void set_batch(Batch &B, const int64_t *seqs, const int32_t *counts, int32_t n, cudaStream_t s) {
     Cache &c = *B.cache;
     check_error(B);
-    need(n, seqs, "seqs");
-    need(n, counts, "counts");
     if (n > B.max_seqs)
         throw Error(SHIELD_ERR_RANGE, std::to_string(n) + " sequences, more than max_seqs " + std::to_string(B.max_seqs));
     int64_t tokens = 0;
@@ -241,7 +260,6 @@ static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const
     if (tokens > B.max_tokens)
         throw Error(SHIELD_ERR_RANGE, std::to_string(tokens) + " tokens, more than max_tokens " + std::to_string(B.max_tokens));
     DeviceScope scope(c.dev.ordinal);
-    const cudaStream_t s = stream_of(c, stream);
     not_captured(s, "setting a batch");
     Plan plan;
     make_plan(c.book, seqs, counts, n, B.shape, plan);
@@ -276,6 +294,13 @@ static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const
     B.planned = true;
 }
 
+static void batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const int32_t *counts, int32_t n, void *stream) {
+    Batch &B = batch_of(ctx, batch);
+    need(n, seqs, "seqs");
+    need(n, counts, "counts");
+    set_batch(B, seqs, counts, n, stream_of(*B.cache, stream));
+}
+
 // A plan holds while its sequences live and no page has moved.
 static void check_plan(Batch &B) {
     check_error(B);
@@ -304,9 +329,8 @@ static int64_t row_stride(int64_t stride, int64_t width, const void *p, int elt,
     return stride;
 }
 
-static void write_rows(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t type, const void *k, int64_t k_stride,
-                       const void *v, int64_t v_stride, void *stream) {
-    Batch &B = batch_of(ctx, batch);
+static void write_rows(Batch &B, int32_t layer, uint32_t type, const void *k, int64_t k_stride, const void *v,
+                       int64_t v_stride, cudaStream_t s) {
     Cache &c = *B.cache;
     check_plan(B);
     check_layer(c, layer);
@@ -315,7 +339,6 @@ static void write_rows(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t t
     const int64_t width = (int64_t)c.pool.kv_heads * c.pool.dim;
     const int elt = type == SHIELD_TYPE_F32 ? 4 : 2;
     DeviceScope scope(c.dev.ordinal);
-    const cudaStream_t s = stream_of(c, stream);
     const bool cap = capturing(s);
     const int64_t tokens = cap ? B.max_tokens : (int64_t)B.last.slot.size();
     if (tokens == 0) return;
@@ -324,9 +347,8 @@ static void write_rows(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t t
     check(launch_write_rows(c.pool, B.plan, tokens, layer, elt == 4, k, k_stride, v, v_stride, s), "writing rows");
 }
 
-static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q, int64_t q_stride, void *out,
-                   int64_t out_stride, float scale, void *stream) {
-    Batch &B = batch_of(ctx, batch);
+static void attend(Batch &B, int32_t layer, const void *q, int64_t q_stride, void *out, int64_t out_stride, float scale,
+                   cudaStream_t s) {
     Cache &c = *B.cache;
     check_plan(B);
     check_layer(c, layer);
@@ -334,7 +356,6 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     const int64_t width = (int64_t)B.n_heads * c.pool.dim;
     DeviceScope scope(c.dev.ordinal);
     AttendArgs A;
-    const cudaStream_t s = stream_of(c, stream);
     const bool cap = capturing(s);
     if (!cap && B.last.perm.empty()) return;
     A.q_stride = row_stride(q_stride, width, q, 2, "q");
@@ -361,6 +382,14 @@ static void attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q,
     check(launch_attend_tile(A, c.maps, tile, c.dev.sms, s), "attention, many rows");
     check(launch_attend_few(A, few, tile > 0, s), "attention, few rows");
     check(launch_attend_merge(A, join, s), "attention, joining");
+}
+
+void write_layer(Batch &B, int32_t layer, const float *k, const float *v, cudaStream_t s) {
+    write_rows(B, layer, SHIELD_TYPE_F32, k, 0, v, 0, s);
+}
+
+void attend_layer(Batch &B, int32_t layer, const void *q, void *out, float scale, cudaStream_t s) {
+    attend(B, layer, q, 0, out, 0, scale, s);
 }
 
 }  // namespace kv
@@ -492,12 +521,18 @@ shield_status shield_kv_batch_set(shield_ctx *ctx, int64_t batch, const int64_t 
 
 shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t type, const void *k,
                               int64_t k_stride, const void *v, int64_t v_stride, void *stream) {
-    return guarded([&] { kv::write_rows(ctx, batch, layer, type, k, k_stride, v, v_stride, stream); });
+    return guarded([&] {
+        kv::Batch &B = kv::batch_of(ctx, batch);
+        kv::write_rows(B, layer, type, k, k_stride, v, v_stride, kv::stream_of(*B.cache, stream));
+    });
 }
 
 shield_status shield_kv_attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q, int64_t q_stride, void *out,
                                int64_t out_stride, float scale, void *stream) {
-    return guarded([&] { kv::attend(ctx, batch, layer, q, q_stride, out, out_stride, scale, stream); });
+    return guarded([&] {
+        kv::Batch &B = kv::batch_of(ctx, batch);
+        kv::attend(B, layer, q, q_stride, out, out_stride, scale, kv::stream_of(*B.cache, stream));
+    });
 }
 
 }  // extern "C"

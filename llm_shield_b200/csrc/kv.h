@@ -12,14 +12,18 @@
 namespace shield {
 namespace kv {
 
+struct Batch;
+
 struct Cache {
     int64_t id = 0;
     DeviceView dev;
     DevPool pool;
     CUtensorMap maps[2];  // keys, values
     Pool book;
-    bool owns = false;  // the pool's memory is the library's
-    Cache(const Pool &b) : book(b) {}
+    int32_t device = 0;  // index within the context
+    bool owns = false;   // the pool's memory is the library's
+    std::unique_ptr<Batch> model;  // of the model's own forwards
+    explicit Cache(const Pool &b) : book(b) {}
     ~Cache();
 };
 
@@ -42,6 +46,15 @@ struct Batch {
     bool planned = false;
     ~Batch();
 };
+
+// The cache's batch for the model's own forwards, with room for a step of this
+// size (made anew, once the GPU is done with it, when it has to grow).
+Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions);
+// Plans a step on the context's stream; the calls below are one layer of it.
+void set_batch(Batch &B, const int64_t *seqs, const int32_t *counts, int32_t n, cudaStream_t s);
+void write_layer(Batch &B, int32_t layer, const float *k, const float *v, cudaStream_t s);
+void attend_layer(Batch &B, int32_t layer, const void *q, void *out, float scale, cudaStream_t s);
+Cache &cache_of(shield_ctx *ctx, int64_t id);
 
 struct State {
     int64_t next_cache = 1, next_batch = 1;

@@ -118,6 +118,40 @@ __global__ void __launch_bounds__(256) k_write_rows(const DevPool pool, const De
     }
 }
 
+// Four values a thread.
+__global__ void __launch_bounds__(256) k_narrow(const float4 *__restrict__ x, uint2 *__restrict__ y, int64_t n4, bool bf16) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    const float4 v = x[i];
+    y[i] = make_uint2(pack_pair(v.x, v.y, bf16), pack_pair(v.z, v.w, bf16));
+}
+__global__ void __launch_bounds__(256) k_widen(const uint2 *__restrict__ x, float4 *__restrict__ y, int64_t n4, bool bf16) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    const uint2 v = x[i];
+    if (bf16) {
+        y[i] = make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xFFFF0000u), __uint_as_float(v.y << 16),
+                           __uint_as_float(v.y & 0xFFFF0000u));
+    } else {
+        const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+        y[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
+}
+
+cudaError_t launch_narrow(const float *x, void *y, int64_t n, bool bf16, cudaStream_t s) {
+    if (n % 4) return cudaErrorInvalidValue;
+    if (n == 0) return cudaSuccess;
+    k_narrow<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(reinterpret_cast<const float4 *>(x), static_cast<uint2 *>(y), n / 4, bf16);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_widen(const void *x, float *y, int64_t n, bool bf16, cudaStream_t s) {
+    if (n % 4) return cudaErrorInvalidValue;
+    if (n == 0) return cudaSuccess;
+    k_widen<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(static_cast<const uint2 *>(x), reinterpret_cast<float4 *>(y), n / 4, bf16);
+    return cudaGetLastError();
+}
+
 cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t tokens, int32_t layer, bool f32,
                               const void *k, int64_t k_stride, const void *v, int64_t v_stride, cudaStream_t s) {
     const int64_t n = tokens * pool.kv_heads * pool.dim / 8;

@@ -53,6 +53,9 @@ cudaError_t launch_move_pages(const DevPool &pool, const Move *moves, int64_t n,
 // upper bound of later plans' (the kernel stops at the plan's count).
 cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t tokens, int32_t layer, bool f32,
                               const void *k, int64_t k_stride, const void *v, int64_t v_stride, cudaStream_t s);
+// n f32 values rounded to the pool's type, and 16-bit values widened to f32.
+cudaError_t launch_narrow(const float *x, void *y, int64_t n, bool bf16, cudaStream_t s);
+cudaError_t launch_widen(const void *x, float *y, int64_t n, bool bf16, cudaStream_t s);
 // The three attention kernels over `units` work units (or CTAs for as many as a
 // later plan may have: each strides over the plan's own count).
 // beside: launch_attend_tile came just before, and this one may run beside it.

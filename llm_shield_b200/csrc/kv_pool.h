@@ -87,6 +87,20 @@ public:
         }
     }
 
+    // Takes back what the latest extend() of these sequences added. (Plans made
+    // before it still hold.)
+    void undo_extend(const int64_t *ids, const int32_t *count, int32_t n) {
+        for (int32_t i = 0; i < n; i++) {
+            Sequence &s = seqs_.at(ids[i]);
+            s.len -= count[i];
+            while ((int64_t)s.pages.size() > pages_of(s.len)) {
+                const int32_t p = s.pages.back();
+                s.pages.pop_back();
+                if (--ref_[p] == 0) give(p);
+            }
+        }
+    }
+
     // Child i: the first len[i] positions (null: all) of parents[i], sharing
     // its full pages (share) or with a copy of every page.
     void fork(const int64_t *parents, const int32_t *len, int32_t n, bool share, int64_t *out, std::vector<Move> &moves) {
