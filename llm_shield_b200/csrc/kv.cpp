@@ -166,7 +166,9 @@ static std::unique_ptr<Batch> make_batch(Cache &c, const shield_kv_batch_config 
     S.max_segments = 2 * n;
     S.max_part = std::min<int64_t>(262144, 16 * T * cfg->n_heads + 16384);
     S.max_table = n * ((cfg->max_positions + (int64_t)c.pool.page_tokens - 1) / c.pool.page_tokens);
-    if (T * S.group > (1 << 30) || S.max_table > (1 << 30)) throw Error(SHIELD_ERR_RANGE, "the batch is too large");
+    // (the kernels count items times kv heads, and a round beyond, in 32 bits)
+    if (T * S.group > (1 << 30) || S.max_table > (1 << 30) || S.max_items * S.kv_heads > (1 << 30))
+        throw Error(SHIELD_ERR_RANGE, "the batch is too large");
     size_t at = 0;
     auto place = [&](size_t count, size_t size) {
         const size_t p = at;

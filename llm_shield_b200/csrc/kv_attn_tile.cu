@@ -214,6 +214,12 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
     return mul2(p, pack2u((uint32_t)t << 23, (uint32_t)(t >> 32) << 23));
 }
 
+// Waits for a phase, 2^22 polls at most: some seconds, a poll lasting up to a
+// few microseconds where it has to wait. (Watching the clock instead cost 5%.)
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity, volatile int *stop, int32_t *err) {
+    return mbar_wait_warp<(1u << 22)>(bar, parity, stop, err);
+}
+
 template <bool BF16, int D>
 __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_constant__ TileArgs args) {
     using S = TileShape<D>;
@@ -299,7 +305,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     const int s = slot % S::STAGES;
                     const int half = lane % S::HALVES, page = lane / S::HALVES, at = b * per + page - window;
                     const int x = __shfl_sync(0xffffffffu, here, at & 31), y = __shfl_sync(0xffffffffu, next, at & 31);
-                    if (!mbar_wait_warp_timed(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
+                    if (!arrived(empty(s), ((slot / S::STAGES) & 1) ^ 1, stop, A.err)) return false;
                     const int pages = min(per, npages - b * per);
                     if (lane == 0) mbar_expect_tx(full(s), (uint32_t)pages * P.page_tokens * D * 2);
                     __syncwarp();
@@ -354,7 +360,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 auto pass = [&](uint32_t slot) {
                     for (; seen != slot; seen++) {
                         const uint32_t s = seen % S::STAGES;
-                        if (!mbar_wait_warp_timed(full(s), (seen / S::STAGES) & 1, stop, A.err)) return false;
+                        if (!arrived(full(s), (seen / S::STAGES) & 1, stop, A.err)) return false;
                         if (leader) mbar_arrive(empty(s));
                         __syncwarp();
                     }
@@ -363,7 +369,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 auto filled = [&](uint32_t slot) {
                     if (!pass(slot)) return false;
                     seen++;
-                    return mbar_wait_warp_timed(full(slot % S::STAGES), (slot / S::STAGES) & 1, stop, A.err);
+                    return arrived(full(slot % S::STAGES), (slot / S::STAGES) & 1, stop, A.err);
                 };
                 auto scores = [&](int n, int h) {  // of half h of this tile's n-th block
                     const uint32_t slot = U.key_slot(b0 + n * step), s = slot % S::STAGES;
@@ -398,8 +404,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     const bool masked = h == 0 && b0 + n * step >= U.clean;
                     if (masked && (!U.wide || a == 0) && leader) mbar_arrive(v_here(a));
                     __syncwarp();
-                    if (masked && U.wide && a == 1 && !mbar_wait_warp_timed(v_clean, cleaned++ & 1, stop, A.err)) return false;
-                    if (!mbar_wait_warp_timed(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
+                    if (masked && U.wide && a == 1 && !arrived(v_clean, cleaned++ & 1, stop, A.err)) return false;
+                    if (!arrived(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
                     tc_fence_after();
                     if (leader) {
 #pragma unroll
@@ -417,7 +423,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     __syncwarp();
                     return true;
                 };
-                ok = mbar_wait_warp_timed(q_full, turn & 1, stop, A.err);
+                ok = arrived(q_full, turn & 1, stop, A.err);
                 if (nblocks > 0) ok = ok && scores(0, 0) && scores(0, 1);
                 // A half's next scores follow its weights' product, whose operand they
                 // overwrite; the other half's are there already, so the softmax finds
@@ -446,7 +452,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     const int rr = U.it.r0 + min(lane + 32 * j, U.it.nr - 1);
                     off[j] = A.plan.perm[U.it.tok0 + rr / A.group] * A.q_stride + (U.kvh * A.group + rr % A.group) * D;
                 }
-                ok = mbar_wait_warp_timed(q_free, (turn & 1) ^ 1, stop, A.err);
+                ok = arrived(q_free, (turn & 1) ^ 1, stop, A.err);
                 if (!ok) break;
                 const int c = lane % VEC;
                 const uint32_t dst = base + (c >> 3) * S::PANEL;
@@ -501,7 +507,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
 #pragma unroll 1
                 for (int h = 0; h < 2; h++) {
-                    if (!mbar_wait_warp_timed(s_full(a, h), (done + n) & 1, stop, A.err)) {
+                    if (!arrived(s_full(a, h), (done + n) & 1, stop, A.err)) {
                         ok = false;
                         break;
                     }
@@ -511,7 +517,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                         // not finite counts as 0 here, and rows that do see such a value get it
                         // at the end.
                         const uint32_t s = U.value_slot(b) % S::STAGES;
-                        if (!mbar_wait_warp_timed(v_here(a), looked++ & 1, stop, A.err)) {
+                        if (!arrived(v_here(a), looked++ & 1, stop, A.err)) {
                             ok = false;
                             break;
                         }
@@ -570,7 +576,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                             if (n > 0 || h > 0) {
                                 // O is still once the previous half's product is done (the one
                                 // before that is: these scores came after it)
-                                if (!mbar_wait_warp_timed(pv_done(a), (h + 1) & 1, stop, A.err)) {
+                                if (!arrived(pv_done(a), (h + 1) & 1, stop, A.err)) {
                                     ok = false;
                                     break;
                                 }
@@ -608,13 +614,13 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 }
             }
             // ---------------------------------------------------- epilogue
-            if (ok && nblocks > 0) ok = mbar_wait_warp_timed(o_full(a), ends & 1, stop, A.err);
+            if (ok && nblocks > 0) ok = arrived(o_full(a), ends & 1, stop, A.err);
             const bool two = U.two();
             if (two) {
                 if (a == 1) {
                     // no product reads the queries any more once tile 0 is done too:
                     // their place takes this tile's outputs, a row a thread
-                    if (ok) ok = mbar_wait_warp_timed(join_ready, joins & 1, stop, A.err);
+                    if (ok) ok = arrived(join_ready, joins & 1, stop, A.err);
                     if (ok && live) {
                         tc_fence_after();
 #pragma unroll 1

@@ -65,34 +65,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // The same kind of bounded wait for a whole warp: every lane polls and a
 // vote makes the outcome warp-uniform, so a loop around it needs no
-// reconvergence point. It gives up after 2^26 polls (a quarter of a second
-// or more; a preempted CTA does not poll, so time it is not running does not
-// count), raising the abort flag and the error word.
+// reconvergence point. It gives up after POLLS polls (2^26: a quarter of a
+// second or more; a preempted CTA does not poll, so time it is not running does
+// not count), raising the abort flag and the error word.
+template <uint32_t POLLS = 1u << 26>
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
     for (uint32_t i = 0;; i++) {
         if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
         if ((i & 255) == 255) {
-            int stop = *abort_flag ? 1 : (i >= (1u << 26) ? 2 : 0);
-            stop = __shfl_sync(0xffffffffu, stop, 0);
-            if (stop) {
-                if (stop == 2 && (threadIdx.x & 31) == 0) {
-                    *abort_flag = 1;
-                    if (err) atomicExch(err, 3);
-                }
-                return false;
-            }
-        }
-    }
-}
-
-// As mbar_wait_warp, bounded by time: about 2 s of SM clock.
-__device__ __forceinline__ bool mbar_wait_warp_timed(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
-    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-    const long long t0 = clock64();
-    for (uint32_t i = 0;; i++) {
-        if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
-        if ((i & 63) == 63) {
-            int stop = *abort_flag ? 1 : (clock64() - t0 > 4000000000LL ? 2 : 0);
+            int stop = *abort_flag ? 1 : (i >= POLLS ? 2 : 0);
             stop = __shfl_sync(0xffffffffu, stop, 0);
             if (stop) {
                 if (stop == 2 && (threadIdx.x & 31) == 0) {

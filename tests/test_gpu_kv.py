@@ -589,3 +589,30 @@ def test_more_work_than_the_gpu_holds_at_once(shape):
         c.k.add_(0)  # something else in between
         c.ctx.kv_attend(b, 1, q.data_ptr(), o.data_ptr(), dim ** -0.5, stream=c.stream)
     assert torch.equal(outs, outs[:1].expand_as(outs)) and first.shape == outs[0].shape
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("new", [1, 2])
+def test_short_pieces_that_a_warp_takes_alone(type, new):
+    """More short sequences than the GPU holds CTAs, behind a prefix and without, with what their rows may not see."""
+    c = Cache(type, 1, 8, 128, 16, pages=900)
+    (root,) = c.ctx.kv_open(c.kv, 1)
+    c.ctx.kv_extend(c.kv, [root], [700])
+    kids = c.ctx.kv_fork(c.kv, [root] * 60, stream=c.stream)
+    c.ctx.kv_extend(c.kv, kids, [new + i % 45 for i in range(60)])
+    lone = c.ctx.kv_open(c.kv, 30)
+    c.ctx.kv_extend(c.kv, lone, [new + 2 * i for i in range(30)])
+    seqs = np.concatenate([kids, lone])
+    check(c, seqs, [new] * 90, 32, layer=0)
+    if new > 1:  # an infinite value at a sequence's end: its last row has it, the rows before do not
+        pages, lens = c.ctx.kv_pages(c.kv, seqs), c.ctx.kv_lengths(c.kv, seqs)
+        for i in range(0, 90, 7):
+            p = int(lens[i]) - 1
+            c.v[0, int(pages[i][p // 16]), 3, p % 16, 5] = math.inf
+        b = c.batch(seqs, [new] * 90, 32)
+        q = torch.randn(90 * new, 32, 128, device="cuda").to(c.dtype)
+        out = torch.empty_like(q)
+        c.ctx.kv_attend(b, 0, q.data_ptr(), out.data_ptr(), 128 ** -0.5, stream=c.stream)
+        hit = torch.zeros_like(out, dtype=torch.bool)
+        hit.view(90, new, 32, 128)[::7, -1, 12:16, 5] = True
+        assert torch.equal(~torch.isfinite(out), hit) and (out[hit] == math.inf).all()
