@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <unordered_set>
 
 #include "kv.h"
 #include "ops.h"
@@ -29,12 +30,9 @@ Batch::~Batch() {
             cudaEventSynchronize(sent[i]);
             cudaEventDestroy(sent[i]);
         }
-        if (host[i]) cudaFreeHost(host[i]);
     }
+    if (host[0]) cudaFreeHost(host[0]);
     cudaFree(dev);
-    cudaFree(part_o);
-    cudaFree(part_ml);
-    if (err) cudaFreeHost(err);
     if (before >= 0) cudaSetDevice(before);
 }
 
@@ -97,7 +95,8 @@ static void create(shield_ctx *ctx, int32_t device, const shield_kv_config *cfg,
     DeviceScope scope(dev.ordinal);
     State &S = kv_state(ctx);
     const int64_t id = S.next_cache;
-    auto cache = std::make_unique<Cache>(Pool(c.n_pages, c.page_tokens, (id << 32) + 1));
+    if (id >= 1 << 18) throw Error(SHIELD_ERR_RANGE, "the context has made too many caches");  // ids hold 18 bits of it
+    auto cache = std::make_unique<Cache>(Pool(c.n_pages, c.page_tokens, id));
     cache->id = id;
     cache->dev = dev;
     cache->device = device;
@@ -181,15 +180,14 @@ static std::unique_ptr<Batch> make_batch(Cache &c, const shield_kv_batch_config 
                  o_merge = place((size_t)T, sizeof(Join)), o_where = place((size_t)S.max_items, 4),
                  o_table = place((size_t)S.max_table, 4);
     B->bytes = at;
+    const size_t o_part = place((size_t)S.max_part * c.pool.dim, 4), o_ml = place((size_t)S.max_part, sizeof(float2));
     SHIELD_CUDA(cudaMalloc(&B->dev, at));
-    for (int i = 0; i < 2; i++) {
-        SHIELD_CUDA(cudaMallocHost(&B->host[i], at));
-        SHIELD_CUDA(cudaEventCreateWithFlags(&B->sent[i], cudaEventDisableTiming));
-    }
-    SHIELD_CUDA(cudaMalloc(&B->part_o, (size_t)S.max_part * c.pool.dim * 4));
-    SHIELD_CUDA(cudaMalloc(&B->part_ml, (size_t)S.max_part * sizeof(float2)));
-    SHIELD_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&B->err), 4, cudaHostAllocMapped));
+    // two images of the plan, and the error word
+    SHIELD_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&B->host[0]), 2 * B->bytes + 4, cudaHostAllocMapped));
+    B->host[1] = B->host[0] + B->bytes;
+    B->err = reinterpret_cast<int32_t *>(B->host[0] + 2 * B->bytes);
     *B->err = 0;
+    for (auto &e : B->sent) SHIELD_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
     SHIELD_CUDA(cudaMemset(B->dev, 0, COUNTS * 4));  // no work until a plan is set
     auto ints = [&](size_t o) { return reinterpret_cast<const int32_t *>(B->dev + o); };
     DevPlan &P = B->plan;
@@ -203,8 +201,8 @@ static std::unique_ptr<Batch> make_batch(Cache &c, const shield_kv_batch_config 
     P.merge = reinterpret_cast<const Join *>(B->dev + o_merge);
     P.where = ints(o_where);
     P.table = ints(o_table);
-    P.part_o = B->part_o;
-    P.part_ml = B->part_ml;
+    P.part_o = reinterpret_cast<float *>(B->dev + o_part);
+    P.part_ml = reinterpret_cast<float2 *>(B->dev + o_ml);
     return B;
 }
 

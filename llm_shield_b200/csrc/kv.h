@@ -31,13 +31,11 @@ struct Batch {
     Cache *cache = nullptr;
     int32_t n_heads = 0, max_tokens = 0, max_seqs = 0, max_positions = 0;
     PlanShape shape;
-    char *dev = nullptr;          // every array of the plan at a fixed offset
-    char *host[2] = {nullptr, nullptr};  // pinned images of it, used in turn
+    char *dev = nullptr;                 // every array of the plan at a fixed offset, then the partials
+    char *host[2] = {nullptr, nullptr};  // pinned images of the plan, used in turn (one allocation)
     cudaEvent_t sent[2] = {nullptr, nullptr};
     int turn = 0;
-    size_t bytes = 0;
-    float *part_o = nullptr;
-    float2 *part_ml = nullptr;
+    size_t bytes = 0;             // of the plan
     int32_t *err = nullptr;       // error word of the kernels' bounded waits, in mapped host memory
     DevPlan plan;
     Plan last;                    // what was uploaded

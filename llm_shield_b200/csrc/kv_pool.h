@@ -11,9 +11,9 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <deque>
 #include <string>
 #include <unordered_map>
-#include <unordered_set>
 #include <vector>
 
 #include "error.h"
@@ -33,8 +33,10 @@ struct Sequence {
 
 class Pool {
 public:
-    Pool(int32_t n_pages, int32_t page_tokens, int64_t first_id)
-        : page_tokens_(page_tokens), free_count_(n_pages), next_id_(first_id), ref_(n_pages, 0),
+    // `number` tells this pool's sequences from other pools': it is the upper
+    // bits of their ids.
+    Pool(int32_t n_pages, int32_t page_tokens, int64_t number)
+        : page_tokens_(page_tokens), free_count_(n_pages), number_(number), ref_(n_pages, 0),
           free_((size_t)(n_pages + 63) / 64, 0) {
         for (int32_t p = 0; p < n_pages; p++) free_[p >> 6] |= uint64_t(1) << (p & 63);
     }
@@ -42,7 +44,7 @@ public:
     int32_t page_tokens() const { return page_tokens_; }
     int32_t n_pages() const { return (int32_t)ref_.size(); }
     int32_t pages_used() const { return n_pages() - free_count_; }
-    int32_t sequences() const { return (int32_t)seqs_.size(); }
+    int32_t sequences() const { return (int32_t)(slots_.size() - idle_.size()); }
     // One past the highest page in use.
     int32_t pages_spanned() const {
         int32_t p = n_pages();
@@ -54,18 +56,12 @@ public:
     int64_t frees() const { return frees_; }
     int64_t moves() const { return moves_; }
 
-    const Sequence &get(int64_t id) const {
-        auto it = seqs_.find(id);
-        if (it == seqs_.end()) throw Error(SHIELD_ERR_ARG, "unknown sequence " + std::to_string(id) + " of this pool");
-        return it->second;
-    }
-    bool has(int64_t id) const { return seqs_.count(id) != 0; }
+    const Sequence &get(int64_t id) const { return slot(id).s; }
+    bool has(int64_t id) const { return find(id) != nullptr; }
 
     void open(int32_t n, int64_t *out) {
-        for (int32_t i = 0; i < n; i++) {
-            seqs_.emplace(next_id_, Sequence());
-            out[i] = next_id_++;
-        }
+        room(n);
+        for (int32_t i = 0; i < n; i++) out[i] = begin();
     }
 
     // Adds count[i] positions to sequence ids[i]; all of them or none.
@@ -81,7 +77,7 @@ public:
         }
         reserve(need);
         for (int32_t i = 0; i < n; i++) {
-            Sequence &s = seqs_.at(ids[i]);
+            Sequence &s = slot(ids[i]).s;
             s.len += count[i];
             while ((int64_t)s.pages.size() < pages_of(s.len)) s.pages.push_back(take());
         }
@@ -91,7 +87,7 @@ public:
     // before it still hold.)
     void undo_extend(const int64_t *ids, const int32_t *count, int32_t n) {
         for (int32_t i = 0; i < n; i++) {
-            Sequence &s = seqs_.at(ids[i]);
+            Sequence &s = slot(ids[i]).s;
             s.len -= count[i];
             while ((int64_t)s.pages.size() > pages_of(s.len)) {
                 const int32_t p = s.pages.back();
@@ -114,11 +110,13 @@ public:
             need += share ? (l % page_tokens_ != 0) : pages_of(l);
         }
         reserve(need);
+        room(n);
         moves.reserve((size_t)need);
-        seqs_.reserve(seqs_.size() + (size_t)n);  // parents stay where they are
         for (int32_t i = 0; i < n; i++) {
-            const Sequence &s = seqs_.at(parents[i]);
-            Sequence c;
+            const int64_t child = begin();
+            const Sequence &s = slot(parents[i]).s;  // (slots stay where they are)
+            Sequence &c = slot(child).s;
+            out[i] = child;
             c.len = len ? len[i] : s.len;
             c.pages.reserve((size_t)pages_of(c.len) + 1);
             for (int32_t j = 0; j < pages_of(c.len); j++) {
@@ -132,8 +130,6 @@ public:
                     c.pages.push_back(p);
                 }
             }
-            out[i] = next_id_++;
-            seqs_.emplace(out[i], std::move(c));
         }
     }
 
@@ -141,10 +137,14 @@ public:
         distinct(ids, n);
         for (int32_t i = 0; i < n; i++) get(ids[i]);
         for (int32_t i = 0; i < n; i++) {
-            auto it = seqs_.find(ids[i]);
-            for (int32_t p : it->second.pages)
+            Slot &t = slot(ids[i]);
+            for (int32_t p : t.s.pages)
                 if (--ref_[p] == 0) give(p);
-            seqs_.erase(it);
+            t.s.pages.clear();  // keeps its memory for the slot's next sequence
+            t.s.len = 0;
+            t.live = false;
+            t.turn = (t.turn + 1) & TURN_MASK;
+            idle_.push_back((int32_t)(ids[i] & SLOT_MASK));
         }
         if (n > 0) frees_++;
     }
@@ -155,7 +155,6 @@ public:
     void compact(std::vector<Move> &moves) {
         std::vector<int32_t> to((size_t)n_pages(), -1);
         int32_t lo = 0, hi = n_pages() - 1;
-        std::vector<size_t> at;  // a moved page's index in moves
         for (;;) {
             while (lo < hi && ref_[lo] != 0) lo++;
             while (hi > lo && ref_[hi] == 0) hi--;
@@ -166,8 +165,8 @@ public:
             hi--;
         }
         if (moves.empty()) return;
-        for (auto &kv : seqs_) {
-            Sequence &s = kv.second;
+        for (Slot &t : slots_) {
+            Sequence &s = t.s;  // (an idle slot has no pages)
             for (int32_t j = 0; j < (int32_t)s.pages.size(); j++) {
                 const int32_t m = to[s.pages[j]];
                 if (m < 0) continue;
@@ -204,21 +203,65 @@ private:
         hint_ = std::min(hint_, (size_t)(p >> 6));
         free_count_++;
     }
-    static void distinct(const int64_t *ids, int32_t n) {
+    void distinct(const int64_t *ids, int32_t n) const {
         if (n < 2) return;
-        std::unordered_set<int64_t> seen;
-        seen.reserve((size_t)n);
-        for (int32_t i = 0; i < n; i++)
-            if (!seen.insert(ids[i]).second)
+        call_++;
+        for (int32_t i = 0; i < n; i++) {
+            const Slot &t = slot(ids[i]);
+            if (t.call == call_)
                 throw Error(SHIELD_ERR_ARG, "sequence " + std::to_string(ids[i]) + " appears twice in one call");
+            t.call = call_;
+        }
+    }
+
+    // An id is the pool's number, the turn of its slot (how many sequences that
+    // had before) and the slot.
+    static constexpr int SLOT_BITS = 22, TURN_BITS = 22;
+    static constexpr int64_t SLOT_MASK = (1 << SLOT_BITS) - 1, TURN_MASK = (1 << TURN_BITS) - 1;
+    struct Slot {
+        Sequence s;
+        int64_t turn = 0;
+        bool live = false;
+        mutable uint64_t call = 0;  // the last call that named it (distinct)
+    };
+    const Slot *find(int64_t id) const {
+        const int64_t at = id & SLOT_MASK;
+        if (id >> (SLOT_BITS + TURN_BITS) != number_ || at >= (int64_t)slots_.size()) return nullptr;
+        const Slot &t = slots_[(size_t)at];
+        return t.live && t.turn == ((id >> SLOT_BITS) & TURN_MASK) ? &t : nullptr;
+    }
+    const Slot &slot(int64_t id) const {
+        const Slot *t = find(id);
+        if (!t) throw Error(SHIELD_ERR_ARG, "unknown sequence " + std::to_string(id) + " of this pool");
+        return *t;
+    }
+    Slot &slot(int64_t id) { return const_cast<Slot &>(const_cast<const Pool *>(this)->slot(id)); }
+    void room(int32_t n) const {
+        if ((int64_t)slots_.size() - (int64_t)idle_.size() + n > SLOT_MASK + 1)
+            throw Error(SHIELD_ERR_NOMEM, "more sequences than a pool takes");
+    }
+    int64_t begin() {  // an empty sequence; room() came first
+        int64_t at;
+        if (idle_.empty()) {
+            at = (int64_t)slots_.size();
+            slots_.emplace_back();
+        } else {
+            at = idle_.back();
+            idle_.pop_back();
+        }
+        Slot &t = slots_[(size_t)at];
+        t.live = true;
+        return number_ << (SLOT_BITS + TURN_BITS) | t.turn << SLOT_BITS | at;
     }
 
     int32_t page_tokens_, free_count_;
-    int64_t next_id_, frees_ = 0, moves_ = 0;
+    int64_t number_, frees_ = 0, moves_ = 0;
+    mutable uint64_t call_ = 0;
     std::vector<int32_t> ref_;     // sequences holding each page
     std::vector<uint64_t> free_;   // one bit per page
     size_t hint_ = 0;              // no free page in a word before this one
-    std::unordered_map<int64_t, Sequence> seqs_;
+    std::deque<Slot> slots_;
+    std::vector<int32_t> idle_;    // slots without a sequence
 };
 
 // ------------------------------------------------------------- attention plan

@@ -28,7 +28,7 @@ static int32_t run(Host *h, F &&f) {
 
 extern "C" {
 
-Host *host_new(int32_t pages, int32_t page_tokens) { return new Host{Pool(pages, page_tokens, (int64_t(1) << 32) + 1), {}, {}, "", 0}; }
+Host *host_new(int32_t pages, int32_t page_tokens) { return new Host{Pool(pages, page_tokens, 1), {}, {}, "", 0}; }
 void host_delete(Host *h) { delete h; }
 const char *host_error(Host *h) { return h->error.c_str(); }
 int32_t host_open(Host *h, int32_t n, int64_t *out) { return run(h, [&] { h->pool.open(n, out); }); }

@@ -234,6 +234,12 @@ def test_refusals_change_nothing(host):
         assert [(H.length(i), H.pages(i)) for i in (a, b)] == before and host.host_used(H.h) == 3
     H.extend([a, b], [0, 0])
     assert host.host_used(H.h) == 3
+    H.free([a])  # an ended sequence's id does not name the next one in its place
+    (c,) = H.open(1).tolist()
+    assert c != a
+    with pytest.raises(binding.ShieldError):
+        H.extend([a], [1])
+    H.extend([c], [1])
 
 
 def check_plan(H, ids, counts, P, group, kv_heads):
