@@ -49,7 +49,9 @@ struct FewShape {
     static constexpr int TILE_BYTES = KEYS * D * 2;
     static constexpr int STAGE_BYTES = 2 * TILE_BYTES;  // keys, values
     static constexpr int RING_BYTES = WARPS * STAGES * STAGE_BYTES;
-    static constexpr int JOIN_BYTES = WARPS * 16 * D * 4;
+    static constexpr int JOIN_LD = D + 8;  // floats from row to row of a warp's output: no bank conflicts
+    static constexpr int JOIN_BYTES = WARPS * 16 * JOIN_LD * 4;
+    static_assert(16 * JOIN_LD * 4 <= STAGES * STAGE_BYTES, "a lone warp's output takes its ring's place");
     static constexpr int BYTES = RING_BYTES > JOIN_BYTES ? RING_BYTES : JOIN_BYTES;
 };
 
@@ -78,9 +80,22 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
         const int ntiles = (it.k1 - it.k0 + S::KEYS - 1) / S::KEYS;
         if (threadIdx.x == 0 && !solo) dirty = 0;
 
+        // The page list in registers, a page per lane, 32 pages and the next 32, so
+        // that no load waits for its page number.
+        const int32_t *const list = table + (it.k0 >> P.page_shift);
+        const int npages = (it.k1 - it.k0 + P.page_tokens - 1) >> P.page_shift;
+        int window = 0;
+        int here = lane < npages ? list[lane] : 0, next = 32 + lane < npages ? list[32 + lane] : 0;
         auto load = [&](int t, int stage) {
             const int p0 = it.k0 + t * S::KEYS;
-            const int64_t off = row_offset(P, A.layer, table[p0 >> P.page_shift], kvh, p0 & (P.page_tokens - 1));
+            int pg = (t * S::KEYS >> P.page_shift) - window;
+            if (pg >= 32) {  // (a warp's tiles are less than 32 pages apart)
+                pg -= 32;
+                window += 32;
+                here = next;
+                next = window + 32 + lane < npages ? list[window + 32 + lane] : 0;
+            }
+            const int64_t off = row_offset(P, A.layer, __shfl_sync(0xffffffffu, here, pg), kvh, p0 & (P.page_tokens - 1));
             const uint16_t *k = static_cast<const uint16_t *>(P.k) + off, *v = static_cast<const uint16_t *>(P.v) + off;
             const uint32_t dst = ring + stage * S::STAGE_BYTES;
 #pragma unroll
@@ -117,6 +132,9 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                 qf[kk][2 + e] = q ? *reinterpret_cast<const uint32_t *>(q + kk * 16 + 8) : 0;
             }
         }
+        // the token whose row this thread helps to write at the end
+        const int mine = solo ? min(lane, it.nr - 1) : min((int)threadIdx.x >> 3, it.nr - 1);
+        const int token = A.plan.perm[it.tok0 + (it.r0 + mine) / A.group];
         const int low = it.masked ? A.plan.lim[it.tok0 + it.r0 / A.group] : it.k1;  // below it every row sees every key
 
         float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
@@ -209,10 +227,9 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
             sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], 2);
         }
         // Writes four dims of a row, which the warps' outputs add up to.
-        auto put = [&](int r, int d, float4 x, float M, float L, bool fix) {
-            const int at = it.tok0 + (it.r0 + r) / A.group, head = kvh * A.group + (it.r0 + r) % A.group;
+        auto put = [&](int r, int tok, int d, float4 x, float M, float L, bool fix) {
             if (fix) {
-                const int end = min(it.k1, A.plan.lim[at]);
+                const int end = min(it.k1, A.plan.lim[it.tok0 + (it.r0 + r) / A.group]);
                 for (int p = it.k0 + (max(low - it.k0, 0) / S::KEYS) * S::KEYS; p < end; p++) {
                     const uint16_t *v = static_cast<const uint16_t *>(P.v) +
                         row_offset(P, A.layer, table[p >> P.page_shift], kvh, p & (P.page_tokens - 1)) + d;
@@ -224,7 +241,8 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
             }
             if (it.part < 0) {
                 const float inv = 1.0f / L;
-                uint16_t *out = static_cast<uint16_t *>(A.out) + A.plan.perm[at] * A.out_stride + head * D + d;
+                const int head = kvh * A.group + (it.r0 + r) % A.group;
+                uint16_t *out = static_cast<uint16_t *>(A.out) + tok * A.out_stride + head * D + d;
                 *reinterpret_cast<uint2 *>(out) = make_uint2(H::pack(x.x * inv, x.y * inv), H::pack(x.z * inv, x.w * inv));
             } else {
                 const int64_t part = it.part + (int64_t)kvh * it.nr + r;
@@ -242,13 +260,15 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                 if ((lane & 3) == 0) join_ml[warp][r] = make_float2(m[e], sum[e]);
 #pragma unroll
                 for (int i = 0; i < D / 8; i++)
-                    *reinterpret_cast<float2 *>(join + r * D + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
+                    *reinterpret_cast<float2 *>(join + r * S::JOIN_LD + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * e], o[i][2 * e + 1]);
             }
             __syncwarp();
-            for (int i = lane; i < it.nr * (D / 4); i += 32) {
-                const int r = i / (D / 4), d = i % (D / 4) * 4;
+            for (int i0 = 0; i0 < it.nr * (D / 4); i0 += 32) {
+                const int i = i0 + lane, r = i / (D / 4), d = i % (D / 4) * 4;
+                const int tok = __shfl_sync(0xffffffffu, token, r & 15);
+                if (r >= it.nr) continue;
                 const float2 ml = join_ml[warp][r];
-                put(r, d, *reinterpret_cast<const float4 *>(join + r * D + d), ml.x, ml.y, fix);
+                put(r, tok, d, *reinterpret_cast<const float4 *>(join + r * S::JOIN_LD + d), ml.x, ml.y, fix);
             }
             __syncwarp();  // the ring is free for the next unit
             continue;
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
             if ((lane & 3) == 0) join_ml[warp][r] = make_float2(m[e], sum[e]);
 #pragma unroll
             for (int i = 0; i < D / 8; i++)
-                *reinterpret_cast<float2 *>(join + (warp * 16 + r) * D + i * 8 + (lane & 3) * 2) =
+                *reinterpret_cast<float2 *>(join + (warp * 16 + r) * S::JOIN_LD + i * 8 + (lane & 3) * 2) =
                     make_float2(o[i][2 * e], o[i][2 * e + 1]);
         }
         if (found) dirty = 1;
@@ -283,13 +303,13 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
                 float4 a = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < S::WARPS; i++) {
-                    const float4 x = *reinterpret_cast<const float4 *>(join + (i * 16 + r) * D + d);
+                    const float4 x = *reinterpret_cast<const float4 *>(join + (i * 16 + r) * S::JOIN_LD + d);
                     a.x = __fmaf_rn(x.x, w[i], a.x);
                     a.y = __fmaf_rn(x.y, w[i], a.y);
                     a.z = __fmaf_rn(x.z, w[i], a.z);
                     a.w = __fmaf_rn(x.w, w[i], a.w);
                 }
-                put(r, d, a, M, L, dirty != 0);
+                put(r, token, d, a, M, L, dirty != 0);
             }
         }
         __syncthreads();  // the ring and join_ml are free for the next unit
