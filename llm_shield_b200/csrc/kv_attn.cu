@@ -149,17 +149,24 @@ __global__ void __launch_bounds__(128, 2) k_attend_few(const AttendArgs A) {
             __syncwarp();
             const uint32_t ks = ring + stage * S::STAGE_BYTES, vs = ks + S::TILE_BYTES;
             const int p0 = it.k0 + t * S::KEYS;
-            float c[2][4];
+            // two chains of products per 8 keys, even and odd steps of 16 dims
+            float c[2][4], c1[2][4];
 #pragma unroll
-            for (int j = 0; j < 2; j++) c[j][0] = c[j][1] = c[j][2] = c[j][3] = 0.0f;
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[j][i] = c1[j][i] = 0.0f;
             const int mi = lane >> 3, mr = lane & 7;
 #pragma unroll
             for (int kk = 0; kk < D / 16; kk++) {
                 uint32_t b[4];
                 ldsm4(b, ks + ((mi >> 1) * 8 + mr) * D * 2 + (((2 * kk + (mi & 1)) ^ mr) << 4));
-                H::mma(c[0], qf[kk], b[0], b[1]);
-                H::mma(c[1], qf[kk], b[2], b[3]);
+                H::mma(kk & 1 ? c1[0] : c[0], qf[kk], b[0], b[1]);
+                H::mma(kk & 1 ? c1[1] : c[1], qf[kk], b[2], b[3]);
             }
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) c[j][i] += c1[j][i];
             const bool masked = p0 + S::KEYS > low;
             if (masked) {
                 // values that a row may not see must not reach its product as 0 * inf:
