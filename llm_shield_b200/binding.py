@@ -167,7 +167,12 @@ def _p(a: np.ndarray):
 
 
 def _addr(a: np.ndarray) -> int:
-    return a.__array_interface__["data"][0]
+    """A contiguous array's address, the quick way where numpy lets it be had
+    (a decode step makes several such calls)."""
+    try:
+        return C.addressof(C.c_char.from_buffer(a))
+    except (TypeError, ValueError, BufferError):  # read-only or empty
+        return a.ctypes.data
 
 
 def _kv_stream(stream: int | None):
@@ -404,7 +409,8 @@ class ShieldContext:
             self._most_pages = int(self.kv_lengths(kv, s).max()) // 16 + 1
             return self.kv_pages(kv, s)
         _check(rc)
-        return out[:, :-(-int(lens.max(initial=0)) // self._page_tokens[kv])].copy()
+        most = max(lens.tolist(), default=0) if lens.size <= 64 else int(lens.max())
+        return out[:, :-(-most // self._page_tokens[kv])].copy()
 
     def kv_batch_create(self, kv: int, n_heads: int, max_tokens: int, max_seqs: int, max_positions: int) -> int:
         c = ShieldKvBatchConfig(n_heads, max_tokens, max_seqs, max_positions)

@@ -7,10 +7,12 @@
 //   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
 //   P = 2^(scale S - m), rounded to the cache's type, over S's own TMEM columns
 //   O += P V    tcgen05.mma with P read from TMEM, O (f32) in TMEM
-// The products of one tile run while the other tile's exponentials are taken,
-// so the tensor pipe and the exponential unit (as scarce: 16 per SM and cycle,
-// which is 1024 cycles for the 128 x 128 weights that two products of 512
-// cycles each use) both stay busy. Up to 128 rows there is one row tile and
+// The exponential unit is as scarce as the tensor pipe (16 per SM and cycle:
+// 1024 cycles for the 128 x 128 weights that two products of 512 cycles each
+// use), so a quarter of the exponentials go to the FMA pipe, and a tile's
+// scores come in halves of 64 keys: one half's are there while the other's are
+// turned into weights, which TMEM has no room for at 128 (S, S, O, O fill its
+// 512 columns). Up to 128 rows there is one row tile and
 // the two take alternate key blocks, each with its own (m, sum, O), joined at
 // the end.
 //
@@ -25,6 +27,11 @@
 //                   are done with theirs
 // The grid is persistent, and every role runs on into the next unit as soon as
 // what it needs is there.
+//
+// Measured: 3 prompts of 4096 tokens, 32 query and 8 kv heads of 128, bf16, in
+// 435 us (950 TFLOP/s of causal pairs) at the power cap, 375-400 us cool. No
+// unit is saturated (tensor pipe 56%, exponentials 42%, issue 44%): each
+// softmax warp waits on its own chain, and the clock falls to 1650 MHz.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -41,8 +48,9 @@ namespace kv {
 using namespace tc;
 
 // Three warpgroups. At launch every thread has 168 registers (64,512 in all);
-// the two softmax warpgroups then take 224 each, a row of S needing 128, and
-// the third keeps 56: 256 * 224 + 128 * 56 = 64,512.
+// the two softmax warpgroups then take 224 each (half a row of S and its
+// weights are 96, a row's outputs on their way out 32 more), and the third
+// keeps 56: 256 * 224 + 128 * 56 = 64,512.
 constexpr int TILE_THREADS = 384;
 constexpr int ROWS = 128;      // rows of a tile
 constexpr int BLOCK = 128;     // keys of a block, the step of the ring

@@ -616,3 +616,15 @@ def test_short_pieces_that_a_warp_takes_alone(type, new):
         hit = torch.zeros_like(out, dtype=torch.bool)
         hit.view(90, new, 32, 128)[::7, -1, 12:16, 5] = True
         assert torch.equal(~torch.isfinite(out), hit) and (out[hit] == math.inf).all()
+
+
+@pytest.mark.parametrize("type,dim", [("f16", 128), ("bf16", 64)])
+def test_a_run_of_keys_in_many_pieces(type, dim):
+    """60,000 keys of one kv head: more pieces than a joining warp has lanes, for few rows and for many."""
+    c = Cache(type, 1, 1, dim, 64, pages=1100)
+    (root,) = c.ctx.kv_open(c.kv, 1)
+    c.ctx.kv_extend(c.kv, [root], [60000])
+    check(c, [root], [1], 8, layer=0)
+    kids = c.ctx.kv_fork(c.kv, [root] * 25, stream=c.stream)
+    c.ctx.kv_extend(c.kv, kids, [1 + i for i in range(25)])
+    check(c, kids, [1] * 25, 8, layer=0)

@@ -376,3 +376,12 @@ def test_small_capacities_fall_back_or_refuse(host):
     empty = H.plan([], [])
     assert not empty["few"].size and not empty["tile"].size
     assert not H.plan(kids, [0] * 8)["perm"].size
+
+
+def test_long_runs_are_cut_into_many_pieces(host):
+    H = HostPool(host, 2000, 64)
+    (root,) = H.open(1).tolist()
+    H.extend([root], [60000])
+    P = H.plan([root], [1], group=8, kv_heads=1)
+    assert P["segs"][0][4] > 32
+    check_plan(H, [root], [1], P, 8, 1)
