@@ -233,7 +233,8 @@ shield_status shield_seq_release(shield_ctx *ctx, int64_t seq);
  * use different streams are ordered by the caller (events), a page freed in
  * one call and handed out in the next among them. Device pointers belong to
  * the cache's GPU, whichever device is current; the current device is left as
- * it was.
+ * it was. A device-side wait that gives up in a call here is reported by the
+ * next call on its batch (SHIELD_ERR_TIMEOUT).
  */
 typedef struct shield_kv_config {
     uint32_t type;       /* SHIELD_TYPE_F16 or SHIELD_TYPE_BF16 */

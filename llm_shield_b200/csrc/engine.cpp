@@ -1554,6 +1554,7 @@ static void kv_forward(shield_ctx *handle, Ctx &C, int64_t kv_id, const int64_t 
             packed.assign(ids + offsets[first], ids + offsets[k]);
             full.resize((size_t)(k - first) * V);
             forward_batch(C, d, packed.data(), B, 0, cancel, -1, 0, nullptr, full.data(), false, false, &step);
+            kv::check_error(step);  // the step is over: its stream was waited for
             if (logits) memcpy(logits + (int64_t)first * V, full.data(), full.size() * 4);
         }
     } catch (...) {

@@ -188,7 +188,7 @@ static std::unique_ptr<Batch> make_batch(Cache &c, const shield_kv_batch_config 
     B->err = reinterpret_cast<int32_t *>(B->host[0] + 2 * B->bytes);
     *B->err = 0;
     for (auto &e : B->sent) SHIELD_CUDA(cudaEventCreateWithFlags(&e, cudaEventDisableTiming));
-    SHIELD_CUDA(cudaMemset(B->dev, 0, COUNTS * 4));  // no work until a plan is set
+    // (nothing is launched on the plan's memory before a plan is set)
     auto ints = [&](size_t o) { return reinterpret_cast<const int32_t *>(B->dev + o); };
     DevPlan &P = B->plan;
     P.counts = ints(o_counts);
@@ -231,7 +231,7 @@ Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int3
 }
 
 // The kernels' bounded waits report here; the host sees it at the next call.
-static void check_error(Batch &B) {
+void check_error(Batch &B) {
     const int32_t e = *static_cast<volatile int32_t *>(B.err);
     if (!e) return;
     *B.err = 0;

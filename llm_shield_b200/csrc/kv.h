@@ -52,6 +52,8 @@ Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int3
 void set_batch(Batch &B, const int64_t *seqs, const int32_t *counts, int32_t n, cudaStream_t s);
 void write_layer(Batch &B, int32_t layer, const float *k, const float *v, cudaStream_t s);
 void attend_layer(Batch &B, int32_t layer, const void *q, void *out, float scale, cudaStream_t s);
+// Throws when a wait of the batch's finished work gave up.
+void check_error(Batch &B);
 Cache &cache_of(shield_ctx *ctx, int64_t id);
 
 struct State {
