@@ -40,6 +40,7 @@
 #include "common.cuh"
 #include "kv_half16.cuh"
 #include "kv_ops.h"
+#include "kv_tile_order.h"
 #include "ptx.cuh"
 
 namespace shield {
@@ -182,29 +183,15 @@ __device__ __forceinline__ bool elected() {
 }
 
 // One work unit as every role sees it.
-struct Unit {
+struct Unit : TileOrder {
     Item it;
-    int kvh, nb;     // kv head, key blocks
-    bool wide;       // two row tiles
-    int lead, ahead; // key blocks whose scores run ahead of their weights, and how many there are
-    int clean;       // whole key blocks that no row is masked in
-    uint32_t ring;   // ring slots filled by earlier units
-    __device__ __forceinline__ Unit(const AttendArgs &A, int u, uint32_t ring_) : ring(ring_) {
+    int kvh;  // kv head
+    __device__ __forceinline__ Unit(const AttendArgs &A, int u, uint32_t ring_) {
         it = A.plan.tile[u / A.pool.kv_heads];
         kvh = u % A.pool.kv_heads;
-        nb = (it.k1 - it.k0 + BLOCK - 1) / BLOCK;
-        wide = it.nr > ROWS;
-        lead = wide ? 1 : 2;
-        ahead = min(lead, nb);
         const int low = it.masked ? A.plan.lim[it.tok0 + it.r0 / A.group] : it.k1;  // below it every row sees every key
-        clean = max(low - it.k0, 0) / BLOCK;
+        set((it.k1 - it.k0 + BLOCK - 1) / BLOCK, it.nr > ROWS, max(low - it.k0, 0) / BLOCK, ring_);
     }
-    // The ring's order: the first `ahead` key blocks, then value block i
-    // followed by key block i + lead while there is one.
-    __device__ __forceinline__ uint32_t key_slot(int b) const { return ring + (b < ahead ? b : ahead + 2 * (b - lead) + 1); }
-    __device__ __forceinline__ uint32_t value_slot(int b) const { return ring + ahead + b + min(b, nb - ahead); }
-    __device__ __forceinline__ bool two() const { return !wide && nb > 1; }  // both warpgroups hold part of the same rows
-    __device__ __forceinline__ int blocks_of(int tile) const { return wide ? nb : (nb - tile + 1) / 2; }
 };
 
 // 2^x of a pair on the FMA pipe, for x in [-inf, 127): x = n + f with n the
@@ -267,7 +254,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 mbar_init(p_full(a, h), 4);
             }
             mbar_init(pv_done(a), 1);
-            mbar_init(v_here(a), 1);
+            mbar_init(v_here(a), VALUES_HERE);
             mbar_init(o_full(a), 1);
         }
         for (int s = 0; s < S::STAGES; s++) {
@@ -277,7 +264,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
         mbar_init(v_clean, 4);
         mbar_init(join_ready, 2);
         mbar_init(q_full, 32);
-        mbar_init(q_free, 3);
+        mbar_init(q_free, QUERIES_FREE);
         *stop = *dirty = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -291,9 +278,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
     const uint32_t tmem = uniform(*tmem_slot);  // S and P of tile a's half h at 128 a + 64 h, O at 256 + 128 a
 
     const int units = (A.tile >= 0 ? A.tile : A.plan.counts[COUNT_TILE]) * P.kv_heads;  // the host keeps it, and one more round, below 2^31
-    // A barrier only tells the parity of its phase, so whoever waits on one waits
-    // for each of its phases in turn, and none can pass before all who wait have
-    // seen it: every ring slot is released by both tiles, whoever uses it.
+    // No phase of a barrier may pass before all who wait for it have seen it
+    // (kv_tile_order.h). Two who wait apart from one another: each ring slot
+    // (released by both tiles, whoever uses it), v_clean's phases (the next look
+    // waits for both tiles).
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
@@ -358,12 +346,8 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             for (int i = 0; ok && i * (int)gridDim.x < units; i++, turn++) {
                 if (dealt(i) >= units) break;
                 Unit U(A, dealt(i), ring);
-                U.nb = uniform(U.nb);
-                U.wide = uniform(U.wide) != 0;
-                U.lead = U.wide ? 1 : 2;
-                U.ahead = min(U.lead, U.nb);
-                U.clean = uniform(U.clean);
-                const int nblocks = U.blocks_of(a), b0 = U.wide ? 0 : a, step = U.wide ? 1 : 2;
+                U.set(uniform(U.nb), uniform(U.wide) != 0, uniform(U.clean), ring);
+                const int nblocks = U.blocks_of(a), b0 = U.first_block(a), step = U.block_step();
                 const uint64_t qd = q_desc + (U.wide ? a * (S::SLOT >> 4) : 0);
                 // Goes through the ring up to `slot`, releasing at once what is the
                 // other tile's.
@@ -398,9 +382,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                             if (n == nblocks - 1) {
                                 // The queries' place is free when both tiles and, where two
                                 // warpgroups join their outputs there, these have said so.
-                                umma_commit(q_free);
-                                if (U.wide ? a == 1 : !U.two()) umma_commit(q_free);
-                                if (!U.wide && !U.two()) umma_commit(q_free);
+                                for (int j = U.frees_queries(a); j > 0; j--) umma_commit(q_free);
                             }
                         }
                     }
@@ -412,7 +394,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                     if (h == 0 && !filled(slot)) return false;
                     const uint64_t vd = v_desc + s * (S::SLOT >> 4);
                     const bool masked = h == 0 && b0 + n * step >= U.clean;
-                    if (masked && (!U.wide || a == 0) && leader) mbar_arrive(v_here(a));
+                    if (masked && leader) mbar_arrive(v_here(U.looker(a)), U.says_values_here());
                     __syncwarp();
                     if (masked && U.wide && a == 1 && !arrived(v_clean, cleaned++ & 1, stop, A.err)) return false;
                     if (!arrived(p_full(a, h), (done + n) & 1, stop, A.err)) return false;
@@ -514,14 +496,14 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
             float m = -INFINITY, sum = 0.0f;  // m: what the weights are relative to, in log2
             const int nblocks = U.blocks_of(a);
             for (int n = 0; ok && n < nblocks; n++) {
-                const int b = U.wide ? n : 2 * n + a, p0 = it.k0 + b * BLOCK;
+                const int b = U.first_block(a) + n * U.block_step(), p0 = it.k0 + b * BLOCK;
 #pragma unroll 1
                 for (int h = 0; h < 2; h++) {
                     if (!arrived(s_full(a, h), (done + n) & 1, stop, A.err)) {
                         ok = false;
                         break;
                     }
-                    if (h == 0 && b >= U.clean && (!U.wide || a == 0)) {
+                    if (h == 0 && b >= U.clean && U.looker(a) == a) {
                         // Values that some row may not see must not reach its product as
                         // 0 * inf, nor may what the slot holds behind the last key: what is
                         // not finite counts as 0 here, and rows that do see such a value get it
