@@ -279,9 +279,19 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
 
     const int units = (A.tile >= 0 ? A.tile : A.plan.counts[COUNT_TILE]) * P.kv_heads;  // the host keeps it, and one more round, below 2^31
     // No phase of a barrier may pass before all who wait for it have seen it
-    // (kv_tile_order.h). Two who wait apart from one another: each ring slot
-    // (released by both tiles, whoever uses it), v_clean's phases (the next look
-    // waits for both tiles).
+    // (kv_tile_order.h). What the next phase needs, barrier by barrier:
+    //   q_full      both tiles' product warps; q_free, to which each of them arrives
+    //               after its wait
+    //   q_free      the query warp; the q_full that it tells after its wait
+    //   full        both product warps; empty, to which each of them arrives
+    //   empty       the copying warp; the full that it tells after its wait
+    //   s_full      warpgroup a; a product that waits for all its warps' p_full
+    //   p_full      product warp a; scores that it issues after its wait
+    //   pv_done     warpgroup a, where a maximum grows: p_full as above
+    //   v_here      the looking warpgroup; all its warps' p_full as above
+    //   v_clean     tile 1's product warp; v_here, to which it arrives after its wait
+    //   o_full      warpgroup a; p_full of a later unit
+    //   join_ready  warpgroup 1; p_full of a later unit
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
@@ -417,6 +427,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1) k_attend_tile(const __grid_co
                 };
                 ok = arrived(q_full, turn & 1, stop, A.err);
                 if (nblocks > 0) ok = ok && scores(0, 0) && scores(0, 1);
+                else if (ok && leader) mbar_arrive(q_free, U.frees_queries(a));
                 // A half's next scores follow its weights' product, whose operand they
                 // overwrite; the other half's are there already, so the softmax finds
                 // scores whenever it comes back.

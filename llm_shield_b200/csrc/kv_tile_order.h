@@ -54,8 +54,11 @@ struct TileOrder {
     // Of two tiles each gives one, so the looker cannot finish a second block
     // (v_clean) before tile 1's product warp has waited for the first.
     SHIELD_HD int says_values_here() const { return wide ? 1 : VALUES_HERE; }
-    // Arrivals on q_free with the commit of a tile's last scores.
-    SHIELD_HD int frees_queries(int tile) const { return 1 + (wide ? tile == 1 : !two()) + (!wide && !two()); }
+    // Arrivals of a tile's product warp on q_free: with the commit of its last
+    // scores or, where it has no block, as soon as it has waited for the queries
+    // (q_full), so that the next unit's cannot come before it has seen these. The
+    // third of two() is the softmax's, when the joined outputs have been read.
+    SHIELD_HD int frees_queries(int tile) const { return blocks_of(tile) == 0 ? 1 : wide ? 1 + tile : two() ? 1 : 2; }
 };
 
 }  // namespace kv

@@ -247,6 +247,8 @@ class Model:
             if n_blocks:
                 yield from scores(0, 0)
                 yield from scores(0, 1)
+            else:
+                self.arrive(self.q_free, frees)
             for n in range(n_blocks):
                 for h in range(2):
                     yield from values(n, h)
@@ -345,6 +347,26 @@ def test_the_model_sees_a_look_that_runs_ahead(lib):
     """Values announced by tile 0 alone: its warpgroup may look through two blocks before tile 1 has waited for one."""
     rules = dict(says_values_here=lambda U, a: 0 if U.wide and a == 1 else 1, values_here=1)
     assert "v_clean" in faults(lib, two_tiles, 8, 20, rules=rules, speed=(1.0, 1.3))
+
+
+def mixed(rng):
+    return [rng.choice(((1, False, 1), (1, False, 0), (2, False, 1), (1, True, 1), (rng.randint(2, 9), rng.random() < 0.5, rng.randint(0, 3))))
+            for _ in range(14)]
+
+
+@pytest.mark.parametrize("stages", [4, 8])
+@pytest.mark.parametrize("speed", SPEEDS, ids=str)
+def test_units_of_one_tile_and_two(lib, stages, speed):
+    """One-block units, which tile 1 has no block of, among others."""
+    for kw in (dict(jitter=0.5), dict(grown=(0.0, 1.0)), dict(grown=(1.0, 0.0), jitter=0.5), dict(copy=20, jitter=0.9)):
+        assert faults(lib, mixed, stages, 12, speed=speed, **kw) == {}
+
+
+def test_the_model_sees_queries_that_run_ahead(lib):
+    """A one-block unit's queries released by tile 0 alone: the next unit's may come before tile 1 has waited for these."""
+    rules = dict(frees_queries=lambda U, a: (3 if a == 0 else 0) if U.nb == 1 and not U.wide else U.frees_queries[a])
+    for stages in (4, 8):
+        assert "q_full" in faults(lib, mixed, stages, 40, rules=rules, speed=(1.0, 2.0))
 
 
 def test_ring_slots_are_taken_once_and_in_order(lib):
