@@ -628,3 +628,54 @@ def test_a_run_of_keys_in_many_pieces(type, dim):
     kids = c.ctx.kv_fork(c.kv, [root] * 25, stream=c.stream)
     c.ctx.kv_extend(c.kv, kids, [1 + i for i in range(25)])
     check(c, kids, [1] * 25, 8, layer=0)
+
+
+@pytest.mark.parametrize("shape", [SHAPES[2], SHAPES[3], SHAPES[6]], ids=lambda s: "-".join(map(str, s)))
+def test_more_work_than_the_gpu_holds_at_once_heads_of_64(shape):
+    test_more_work_than_the_gpu_holds_at_once(shape)
+
+
+@pytest.mark.parametrize("shape", [("f16", 64, 64, 8, 8), ("bf16", 64, 16, 4, 16), ("bf16", 128, 64, 8, 8), ("f16", 128, 32, 4, 16)],
+                         ids=lambda s: "-".join(map(str, s)))
+@pytest.mark.parametrize("grows", [(1,), (0,), (0, 1)], ids=["second", "first", "both"])
+def test_tiles_with_unequal_work(shape, grows):
+    """Units of two row tiles, of one and of one key block, where the scores of one tile's rows grow from key to key,
+    so that its maxima grow in every half block, and the other's fall."""
+    type, dim, pt, kv_heads, heads = shape
+    G, rng = heads // kv_heads, random.Random(f"{shape}{grows}")
+    c = Cache(type, 1, kv_heads, dim, pt, pages=-(-40000 // pt))
+    rows = 512 // G
+    before = [0, 0, 700, 100, 129, 1000, 255, 640, 900, 1, 383, 500] + [300] * (148 // kv_heads // 2)
+    counts = [rows - rng.choice((0, 0, 1, 17)) for _ in before]
+    counts += [rng.randint(20 // G + 1, 128 // G) for _ in range(60)]  # one key block, one tile
+    before += [0] * 60
+    counts += [100 // G + 1] * 8
+    before += [rng.randint(100, 400) for _ in range(8)]
+    seqs = c.ctx.kv_open(c.kv, len(counts))
+    c.ctx.kv_extend(c.kv, seqs, [n + m for n, m in zip(before, counts)])
+    # scale q.k is 0.1 a key upwards: 9 in log2 per half block, above the growth that the kernel lets pass
+    sign = torch.randint(0, 2, (dim,), device="cuda", generator=c.gen).mul_(2).sub_(1)
+    step = 0.1 / dim ** 0.5
+    for s, n, m in zip(seqs, before, counts):
+        pages = torch.from_numpy(c.ctx.kv_pages(c.kv, [s])[0]).long().cuda()
+        at = torch.arange(pages.numel() * pt, device="cuda").view(-1, 1, pt, 1)
+        c.k[0, pages] = (c.k[0, pages].float() * 0.05 + at * step * sign).to(c.dtype)
+    q = torch.empty(sum(counts), heads, dim, device="cuda").normal_(0, 0.05, generator=c.gen)
+    t = 0
+    for m in counts:
+        tile = (torch.arange(m, device="cuda") * G // 128) % 2
+        up = sum((tile == g) for g in grows).clamp(max=1)
+        q[t:t + m] += (2 * up - 1)[:, None, None] * sign
+        t += m
+    q = q.to(c.dtype)
+    scale = dim ** -0.5
+    b = c.batch(seqs, counts, heads)
+    outs = torch.empty(6, *q.shape, dtype=c.dtype, device="cuda")
+    for o in outs:
+        c.ctx.kv_attend(b, 0, q.data_ptr(), o.data_ptr(), scale, stream=c.stream)
+    torch.cuda.synchronize()
+    c.ctx.kv_batch_set(b, seqs, counts, stream=c.stream)  # would say so if a wait had given up
+    want, tol = expect(c, seqs, counts, q, 0, scale)
+    worst = ((outs[0].double() - want).abs() / tol).max().item()
+    assert worst <= 1, f"{worst} times the tolerance"
+    assert torch.equal(outs, outs[:1].expand_as(outs))
