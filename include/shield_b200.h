@@ -278,7 +278,8 @@ shield_status shield_kv_copy(shield_ctx *ctx, int64_t kv, const int64_t *seqs, c
 shield_status shield_kv_free(shield_ctx *ctx, int64_t kv, const int64_t *seqs, int32_t n);
 /* Packs the pool: the highest used page moves to the lowest free one, and so
  * on until the used pages are the lowest ones. Sequences keep their contents;
- * batches have to be set again. moved (optional): pages moved. */
+ * batches have to be set again. moved (optional): pages moved. If the call
+ * fails, nothing has changed. */
 shield_status shield_kv_compact(shield_ctx *ctx, int64_t kv, int32_t *moved, void *stream);
 /* lengths[i] (optional): positions sequence seqs[i] holds; pages (optional):
  * its page numbers in pages[i * max_pages ..], padded with -1, SHIELD_ERR_RANGE

@@ -474,8 +474,9 @@ shield_status shield_kv_compact(shield_ctx *ctx, int64_t kv, int32_t *moved, voi
         const cudaStream_t s = kv::stream_of(c, stream);
         kv::not_captured(s, "compacting");
         std::vector<kv::Move> moves;
-        c.book.compact(moves);
+        c.book.plan_compact(moves);
         kv::check(kv::launch_move_pages(c.pool, moves.data(), (int64_t)moves.size(), s), "moving pages");
+        c.book.take_moves(moves);  // only now: sequences keep their pages if a launch fails
         if (moved) *moved = (int32_t)moves.size();
     });
 }

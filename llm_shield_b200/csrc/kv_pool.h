@@ -12,6 +12,7 @@
 
 #include <algorithm>
 #include <deque>
+#include <numeric>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -152,7 +153,9 @@ public:
     // The i-th highest used page moves to the i-th lowest free one while that
     // is lower; afterwards the used pages are the lowest ones. The pages read
     // and the pages written are disjoint, so the moves may run in any order.
-    void compact(std::vector<Move> &moves) {
+    // Nothing changes before take_moves(), when the rows are on their way: until
+    // then what was copied lies in free pages.
+    void plan_compact(std::vector<Move> &moves) const {
         std::vector<int32_t> to((size_t)n_pages(), -1);
         int32_t lo = 0, hi = n_pages() - 1;
         for (;;) {
@@ -165,15 +168,22 @@ public:
             hi--;
         }
         if (moves.empty()) return;
-        for (Slot &t : slots_) {
-            Sequence &s = t.s;  // (an idle slot has no pages)
+        for (const Slot &t : slots_) {
+            const Sequence &s = t.s;  // (an idle slot has no pages)
             for (int32_t j = 0; j < (int32_t)s.pages.size(); j++) {
                 const int32_t m = to[s.pages[j]];
-                if (m < 0) continue;
-                moves[m].rows = std::max(moves[m].rows, std::min(page_tokens_, s.len - j * page_tokens_));
-                s.pages[j] = moves[m].dst;
+                if (m >= 0) moves[m].rows = std::max(moves[m].rows, std::min(page_tokens_, s.len - j * page_tokens_));
             }
         }
+    }
+    // What plan_compact() gave, with no other call in between.
+    void take_moves(const std::vector<Move> &moves) {
+        if (moves.empty()) return;
+        std::vector<int32_t> to((size_t)n_pages());
+        std::iota(to.begin(), to.end(), 0);
+        for (const Move &m : moves) to[m.src] = m.dst;
+        for (Slot &t : slots_)
+            for (int32_t &p : t.s.pages) p = to[p];
         for (const Move &m : moves) {
             std::swap(ref_[m.src], ref_[m.dst]);
             free_[m.dst >> 6] &= ~(uint64_t(1) << (m.dst & 63));
@@ -181,6 +191,10 @@ public:
         }
         hint_ = 0;
         moves_++;
+    }
+    void compact(std::vector<Move> &moves) {
+        plan_compact(moves);
+        take_moves(moves);
     }
 
 private:

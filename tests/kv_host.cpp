@@ -38,6 +38,7 @@ int32_t host_fork(Host *h, const int64_t *ids, const int32_t *len, int32_t n, in
 }
 int32_t host_free(Host *h, const int64_t *ids, int32_t n) { return run(h, [&] { h->pool.free(ids, n); }); }
 int32_t host_compact(Host *h) { return run(h, [&] { h->moves.clear(); h->pool.compact(h->moves); }); }
+int32_t host_plan_compact(Host *h) { return run(h, [&] { h->moves.clear(); h->pool.plan_compact(h->moves); }); }
 int32_t host_moves(Host *h, int32_t *out) {
     if (out && !h->moves.empty()) memcpy(out, h->moves.data(), h->moves.size() * sizeof(Move));
     return (int32_t)h->moves.size();

@@ -3,6 +3,7 @@ and compacted, rows written, and attention over shared and private pages
 against the definition in 64 bits."""
 from __future__ import annotations
 
+import ctypes
 import math
 import random
 
@@ -679,3 +680,44 @@ def test_tiles_with_unequal_work(shape, grows):
     worst = ((outs[0].double() - want).abs() / tol).max().item()
     assert worst <= 1, f"{worst} times the tolerance"
     assert torch.equal(outs, outs[:1].expand_as(outs))
+
+
+class StaleError:
+    """A failed call of the caller's own, whose error the runtime still holds for this thread."""
+
+    def __enter__(self):
+        torch.cuda.synchronize()
+        self.rt = ctypes.CDLL("libcudart.so.12")  # torch's and the library's
+        assert self.rt.cudaSetDevice(1000) != 0 and self.rt.cudaPeekAtLastError() != 0
+
+    def __exit__(self, *_):
+        self.rt.cudaGetLastError()
+
+
+def scattered(c):
+    """501 forks of a root, each with a page of its own, behind 400 free pages, and what they hold."""
+    (root,) = c.ctx.kv_open(c.kv, 1)
+    c.ctx.kv_extend(c.kv, [root], [16 * 10 + 5])
+    want = c.rows(root, 0, c.k).clone()
+    kids = c.ctx.kv_fork(c.kv, [root] * 901, stream=c.stream)
+    gone = c.ctx.kv_pages(c.kv, kids[:400])[:, -1]
+    c.ctx.kv_free(c.kv, kids[:400])
+    c.k[:, torch.from_numpy(gone).long().cuda()] = 9.0
+    return kids[400:], want
+
+
+def test_a_compaction_that_fails_changes_nothing():
+    c = Cache("f16", 1, 1, 64, 16, pages=2000)
+    kids, want = scattered(c)
+    with StaleError():
+        try:
+            c.ctx.kv_compact(c.kv, stream=c.stream)
+        except binding.ShieldError as e:
+            assert e.code == binding.ERR_CUDA
+    for s in kids[::20]:
+        assert torch.equal(c.rows(s, 0, c.k), want)
+    c.ctx.kv_compact(c.kv, stream=c.stream)
+    info = c.ctx.kv_info(c.kv)
+    assert info["pages_spanned"] == info["pages_used"] == 10 + 1 + 501
+    for s in kids:
+        assert torch.equal(c.rows(s, 0, c.k), want)

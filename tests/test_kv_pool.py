@@ -385,3 +385,30 @@ def test_long_runs_are_cut_into_many_pieces(host):
     P = H.plan([root], [1], group=8, kv_heads=1)
     assert P["segs"][0][4] > 32
     check_plan(H, [root], [1], P, 8, 1)
+
+
+@pytest.mark.parametrize("pt", [16, 128])
+def test_a_planned_compaction_changes_nothing_until_it_is_taken(host, pt):
+    rng = random.Random(pt)
+    host.host_plan_compact.argtypes = [C.c_void_p]
+    p = HostPool(host, 300, pt)
+    ids = list(p.open(30))
+    p.extend(ids, [rng.randint(0, 6 * pt) for _ in ids])
+    ids += list(p.fork(ids[:10]))
+    gone = rng.sample(ids, 15)
+    p.free(gone)
+    live = [i for i in ids if i not in gone]
+
+    def state():
+        return [(p.length(i), p.pages(i)) for i in live], host.host_used(p.h), host.host_spanned(p.h)
+
+    before = state()
+    for _ in range(2):
+        p.check(host.host_plan_compact(p.h))
+        assert state() == before
+    p.extend(live[:1], [1])  # pages are handed out as before the plan
+    held = {x for i in live for x in p.pages(i)}
+    p.check(host.host_plan_compact(p.h))
+    planned = p.moves()
+    np.testing.assert_array_equal(p.compact(), planned)
+    assert len(planned) and host.host_spanned(p.h) == host.host_used(p.h) == len(held)
