@@ -12,9 +12,11 @@
 #define SHIELD_CUDA(x)                                                                                 \
     do {                                                                                               \
         cudaError_t e_ = (x);                                                                          \
-        if (e_ != cudaSuccess)                                                                         \
+        if (e_ != cudaSuccess) {                                                                       \
+            cudaGetLastError(); /* reported here: no later launch may take it for its own */           \
             throw ::shield::Error(e_ == cudaErrorMemoryAllocation ? SHIELD_ERR_NOMEM : SHIELD_ERR_CUDA, \
-                                  std::string(#x) + " failed: " + cudaGetErrorString(e_));           \
+                                  std::string(#x) + " failed: " + cudaGetErrorString(e_));             \
+        }                                                                                              \
     } while (0)
 
 namespace shield {

@@ -69,7 +69,9 @@ static void not_captured(cudaStream_t s, const char *what) {
 }
 
 static void check(cudaError_t e, const char *what) {
-    if (e != cudaSuccess) throw Error(SHIELD_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+    if (e == cudaSuccess) return;
+    cudaGetLastError();
+    throw Error(SHIELD_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
 static void need(int32_t n, const void *p, const char *what) {

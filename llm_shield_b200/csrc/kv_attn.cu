@@ -331,7 +331,7 @@ static cudaError_t few_launch(const AttendArgs &A, int64_t units, bool beside, c
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(k_attend_few<BF16, D>, S::BYTES, allowed);
     if (e != cudaSuccess) return e;
-    return launch_early(k_attend_few<BF16, D>, (unsigned)units, 128, S::BYTES, beside, s, A);
+    return launch(k_attend_few<BF16, D>, (unsigned)units, 128, S::BYTES, beside, s, A);
 }
 
 cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, bool beside, cudaStream_t s) {
@@ -417,7 +417,7 @@ __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
 template <bool BF16, int D>
 static cudaError_t merge_launch(const AttendArgs &A, int64_t tokens, cudaStream_t s) {
     const int64_t rows = tokens * A.group * A.pool.kv_heads;
-    return launch_early(k_attend_merge<BF16, D>, (unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 30), 128, 0, true, s, A);
+    return launch(k_attend_merge<BF16, D>, (unsigned)std::min<int64_t>((rows + 3) / 4, 1 << 30), 128, 0, true, s, A);
 }
 
 cudaError_t launch_attend_merge(const AttendArgs &A, int64_t tokens, cudaStream_t s) {

@@ -777,8 +777,7 @@ static cudaError_t tile_launch(const TileArgs &T, int64_t units, int sms, cudaSt
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(k_attend_tile<BF16, D>, S::BYTES, allowed);
     if (e != cudaSuccess) return e;
-    k_attend_tile<BF16, D><<<(unsigned)std::min<int64_t>(units, sms), TILE_THREADS, S::BYTES, s>>>(T);
-    return cudaGetLastError();
+    return launch(k_attend_tile<BF16, D>, (unsigned)std::min<int64_t>(units, sms), TILE_THREADS, S::BYTES, false, s, T);
 }
 
 cudaError_t launch_attend_tile(const AttendArgs &A, const CUtensorMap *maps, int64_t units, int sms, cudaStream_t s) {

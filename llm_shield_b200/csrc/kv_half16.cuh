@@ -7,6 +7,7 @@
 
 #include <atomic>
 
+#include "kv_launch.cuh"
 #include "kv_ops.h"
 
 namespace shield {
@@ -80,24 +81,6 @@ inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t> &done) 
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
     return e;
-}
-
-// A launch that may start while the kernel before it in the stream still runs
-// (early): the kernel itself waits (griddepcontrol.wait) where it needs what
-// that one wrote, and never ends before it.
-template <class K, class... Args>
-inline cudaError_t launch_early(K kernel, unsigned grid, unsigned threads, int smem, bool early, cudaStream_t s, const Args &...args) {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(grid);
-    c.blockDim = dim3(threads);
-    c.dynamicSmemBytes = (size_t)smem;
-    c.stream = s;
-    cudaLaunchAttribute a;
-    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    a.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &a;
-    c.numAttrs = early ? 1 : 0;
-    return cudaLaunchKernelEx(&c, kernel, args...);
 }
 
 // First element of position `row` of a page: layer, page, kv head.

@@ -9,6 +9,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "kv_launch.cuh"
 #include "kv_ops.h"
 
 namespace shield {
@@ -56,8 +57,7 @@ template <int N>
 static cudaError_t move_some(const DevPool &pool, const Move *moves, int n, cudaStream_t s) {
     MoveList<N> list;
     memcpy(list.m, moves, (size_t)n * sizeof(Move));
-    k_move_pages<N><<<dim3((unsigned)n, (unsigned)pool.layers * 2), 256, 0, s>>>(list, pool);
-    return cudaGetLastError();
+    return launch(k_move_pages<N>, dim3((unsigned)n, (unsigned)pool.layers * 2), 256, 0, false, s, list, pool);
 }
 
 cudaError_t launch_move_pages(const DevPool &pool, const Move *moves, int64_t n, cudaStream_t s) {
@@ -143,15 +143,15 @@ __global__ void __launch_bounds__(256) k_widen(const uint2 *__restrict__ x, floa
 cudaError_t launch_narrow(const float *x, void *y, int64_t n, bool bf16, cudaStream_t s) {
     if (n % 4) return cudaErrorInvalidValue;
     if (n == 0) return cudaSuccess;
-    k_narrow<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(reinterpret_cast<const float4 *>(x), static_cast<uint2 *>(y), n / 4, bf16);
-    return cudaGetLastError();
+    return launch(k_narrow, (unsigned)((n / 4 + 255) / 256), 256, 0, false, s, reinterpret_cast<const float4 *>(x), static_cast<uint2 *>(y),
+                  n / 4, bf16);
 }
 
 cudaError_t launch_widen(const void *x, float *y, int64_t n, bool bf16, cudaStream_t s) {
     if (n % 4) return cudaErrorInvalidValue;
     if (n == 0) return cudaSuccess;
-    k_widen<<<(unsigned)((n / 4 + 255) / 256), 256, 0, s>>>(static_cast<const uint2 *>(x), reinterpret_cast<float4 *>(y), n / 4, bf16);
-    return cudaGetLastError();
+    return launch(k_widen, (unsigned)((n / 4 + 255) / 256), 256, 0, false, s, static_cast<const uint2 *>(x), reinterpret_cast<float4 *>(y),
+                  n / 4, bf16);
 }
 
 cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t tokens, int32_t layer, bool f32,
@@ -159,9 +159,7 @@ cudaError_t launch_write_rows(const DevPool &pool, const DevPlan &plan, int64_t 
     const int64_t n = tokens * pool.kv_heads * pool.dim / 8;
     if (n == 0) return cudaSuccess;
     const dim3 grid((unsigned)std::min<int64_t>((n + 1023) / 1024, 1 << 20), 2);
-    if (f32) k_write_rows<true><<<grid, 256, 0, s>>>(pool, plan, layer, k, k_stride, v, v_stride);
-    else k_write_rows<false><<<grid, 256, 0, s>>>(pool, plan, layer, k, k_stride, v, v_stride);
-    return cudaGetLastError();
+    return launch(f32 ? k_write_rows<true> : k_write_rows<false>, grid, 256, 0, false, s, pool, plan, layer, k, k_stride, v, v_stride);
 }
 
 }  // namespace kv

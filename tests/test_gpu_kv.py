@@ -721,3 +721,31 @@ def test_a_compaction_that_fails_changes_nothing():
     assert info["pages_spanned"] == info["pages_used"] == 10 + 1 + 501
     for s in kids:
         assert torch.equal(c.rows(s, 0, c.k), want)
+
+
+def test_errors_of_other_calls_are_not_taken_for_a_launchs_own():
+    """Forks, compactions, writes and attention after a failed allocation of the library's and a failed call of the caller's."""
+    c = Cache("f16", 1, 1, 64, 16, pages=2000)
+    kids, want = scattered(c)
+    rt = ctypes.CDLL("libcudart.so.12")
+    for _ in range(2):
+        with pytest.raises(binding.ShieldError) as e:  # 4 TB
+            c.ctx.kv_create("f16", 1, 128, 128, 128, 1 << 20)
+        assert e.value.code == binding.ERR_NOMEM
+        assert rt.cudaPeekAtLastError() == 0
+        kids = np.concatenate([kids, c.ctx.kv_fork(c.kv, kids[:1], stream=c.stream)])
+    q, out = (torch.zeros(40, 4, 64, dtype=torch.float16, device="cuda") for _ in range(2))
+    new = torch.randn(40, 1, 64, device="cuda")
+    with StaleError():
+        kids = np.concatenate([kids, c.ctx.kv_fork(c.kv, np.repeat(kids[:1], 350), stream=c.stream)])
+        assert c.ctx.kv_compact(c.kv, stream=c.stream) == 400 - 352
+        (s,) = c.ctx.kv_copy(c.kv, kids[-1:], stream=c.stream)
+        c.ctx.kv_extend(c.kv, [s], [40])
+        lens = c.ctx.kv_lengths(c.kv, [s])
+        b = c.ctx.kv_batch_create(c.kv, 4, 40, 1, int(lens[0]))
+        for n in (40, 1):  # the kernel of many rows, the one of few
+            c.ctx.kv_batch_set(b, [s], [n], stream=c.stream)
+            c.ctx.kv_write(b, 0, new[-n:].data_ptr(), new[-n:].data_ptr(), "f32", stream=c.stream)
+            c.ctx.kv_attend(b, 0, q.data_ptr(), out.data_ptr(), 0.125, stream=c.stream)
+    for s in kids:
+        assert torch.equal(c.rows(s, 0, c.k), want)
