@@ -233,8 +233,9 @@ shield_status shield_seq_release(shield_ctx *ctx, int64_t seq);
  * use different streams are ordered by the caller (events), a page freed in
  * one call and handed out in the next among them. Device pointers belong to
  * the cache's GPU, whichever device is current; the current device is left as
- * it was. A device-side wait that gives up in a call here is reported by the
- * next call on its batch (SHIELD_ERR_TIMEOUT).
+ * it was. A device-side wait that gives up (SHIELD_ERR_TIMEOUT) leaves rows of
+ * its call's output undefined; shield_kv_batch_check tells, once the work was
+ * waited for, else the next call on the batch.
  */
 typedef struct shield_kv_config {
     uint32_t type;       /* SHIELD_TYPE_F16 or SHIELD_TYPE_BF16 */
@@ -337,6 +338,11 @@ shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uin
  */
 shield_status shield_kv_attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q, int64_t q_stride, void *out,
                                int64_t out_stride, float scale, void *stream);
+
+/* SHIELD_ERR_TIMEOUT, once, when a device-side wait of the batch's work so far
+ * has given up and no call has said so yet. For a caller that has waited for a
+ * step, a replayed one too, and is about to use its results. */
+shield_status shield_kv_batch_check(shield_ctx *ctx, int64_t batch);
 
 /*
  * shield_seq_forward on sequences of a paged cache of the configured model's
@@ -449,6 +455,10 @@ enum {
  * `layer` copied out to `out`, for layer-by-layer parity checks. */
 shield_status shield_debug_activation(shield_ctx *ctx, int32_t device, const int32_t *ids, int32_t n,
                                       int32_t layer, int32_t what, float *out);
+
+/* Sets the error word of a paged cache's batch (0: of the cache's own forwards)
+ * as a device-side wait that gives up does, for tests of its way to the caller. */
+shield_status shield_debug_kv_error(shield_ctx *ctx, int64_t kv, int64_t batch, int32_t word);
 
 /* Device-side accounting of the context's work, for benchmarks. */
 typedef struct shield_timing {

@@ -82,7 +82,7 @@ EXPORTS = [
     "shield_kv_create", "shield_kv_release", "shield_kv_get_info", "shield_kv_open", "shield_kv_extend",
     "shield_kv_fork", "shield_kv_copy", "shield_kv_free", "shield_kv_compact", "shield_kv_pages",
     "shield_kv_batch_create", "shield_kv_batch_release", "shield_kv_batch_set", "shield_kv_write", "shield_kv_attend",
-    "shield_kv_forward",
+    "shield_kv_batch_check", "shield_kv_forward", "shield_debug_kv_error",
 ]
 
 _lib = None
@@ -141,6 +141,8 @@ def lib() -> C.CDLL:
         L.shield_kv_batch_set.argtypes = [P, I64, P, P, I32, P]
         L.shield_kv_write.argtypes = [P, I64, I32, C.c_uint32, P, I64, P, I64, P]
         L.shield_kv_attend.argtypes = [P, I64, I32, P, I64, P, I64, C.c_float, P]
+        L.shield_kv_batch_check.argtypes = [P, I64]
+        L.shield_debug_kv_error.argtypes = [P, I64, I64, I32]
         L.shield_kv_forward.argtypes = [P, I64, P, P, P, I32, P, P]
         L.shield_last_error.restype = C.c_char_p
         for name in EXPORTS:
@@ -427,6 +429,14 @@ class ShieldContext:
         if s.shape != c.shape or s.ndim != 1:
             raise ValueError("one count per sequence")
         _check(lib().shield_kv_batch_set(self._h, batch, _addr(s), _addr(c), s.size, _kv_stream(stream)))
+
+    def kv_batch_check(self, batch: int) -> None:
+        """Raises when a device-side wait of the batch's finished work gave up."""
+        _check(lib().shield_kv_batch_check(self._h, batch))
+
+    def debug_kv_error(self, kv: int, batch: int, word: int) -> None:
+        """Sets a batch's error word as a wait that gives up does (0: of the cache's own forwards)."""
+        _check(lib().shield_debug_kv_error(self._h, kv, batch, word))
 
     def kv_write(self, batch: int, layer: int, k: int, v: int, type: str, k_stride: int = 0, v_stride: int = 0,
                  stream: int | None = None) -> None:

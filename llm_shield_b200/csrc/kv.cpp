@@ -522,6 +522,19 @@ shield_status shield_kv_batch_set(shield_ctx *ctx, int64_t batch, const int64_t 
     return guarded([&] { kv::batch_set(ctx, batch, seqs, counts, n, stream); });
 }
 
+shield_status shield_kv_batch_check(shield_ctx *ctx, int64_t batch) {
+    return guarded([&] { kv::check_error(kv::batch_of(ctx, batch)); });
+}
+
+shield_status shield_debug_kv_error(shield_ctx *ctx, int64_t kv, int64_t batch, int32_t word) {
+    return guarded([&] {
+        kv::Cache &c = kv::cache_of(ctx, kv);
+        kv::Batch *B = batch ? &kv::batch_of(ctx, batch) : c.model.get();
+        if (!B || B->cache != &c) throw Error(SHIELD_ERR_ARG, "the cache has no such batch");
+        *static_cast<volatile int32_t *>(B->err) = word;
+    });
+}
+
 shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t type, const void *k,
                               int64_t k_stride, const void *v, int64_t v_stride, void *stream) {
     return guarded([&] {

@@ -749,3 +749,31 @@ def test_errors_of_other_calls_are_not_taken_for_a_launchs_own():
             c.ctx.kv_attend(b, 0, q.data_ptr(), out.data_ptr(), 0.125, stream=c.stream)
     for s in kids:
         assert torch.equal(c.rows(s, 0, c.k), want)
+
+
+def test_a_wait_that_gave_up_is_told():
+    """The error word, set from the host as a kernel's wait sets it: told once, by whichever call comes first."""
+    c = Cache("bf16", 1, 2, 64, 16, pages=40)
+    s = c.ctx.kv_open(c.kv, 2)
+    c.ctx.kv_extend(c.kv, s, [30, 5])
+    b, other = (c.batch(s, [3, 1], 4) for _ in range(2))
+    q, out = (torch.zeros(4, 4, 64, dtype=c.dtype, device="cuda") for _ in range(2))
+    k = torch.randn(4, 2, 64, device="cuda")
+    calls = [lambda b: c.ctx.kv_batch_check(b), lambda b: c.ctx.kv_batch_set(b, s, [3, 1], stream=c.stream),
+             lambda b: c.ctx.kv_write(b, 0, k.data_ptr(), k.data_ptr(), "f32", stream=c.stream),
+             lambda b: c.ctx.kv_attend(b, 0, q.data_ptr(), out.data_ptr(), 0.1, stream=c.stream)]
+    for call in calls:
+        call(b)
+    for first in calls:
+        c.ctx.debug_kv_error(c.kv, b, 3)
+        c.ctx.kv_batch_check(other)  # another batch's work
+        with pytest.raises(binding.ShieldError) as e:
+            first(b)
+        assert e.value.code == binding.ERR_TIMEOUT and "gave up" in str(e.value)
+        for call in calls:
+            call(b)
+    far = c.ctx.kv_create("bf16", 1, 2, 64, 16, 4)
+    for bad in (lambda: c.ctx.kv_batch_check(b + 100), lambda: c.ctx.debug_kv_error(far, b, 1), lambda: c.ctx.debug_kv_error(c.kv, 0, 1)):
+        with pytest.raises(binding.ShieldError) as e:
+            bad()
+        assert e.value.code == binding.ERR_ARG
