@@ -1558,6 +1558,7 @@ static void kv_forward(shield_ctx *handle, Ctx &C, int64_t kv_id, const int64_t 
             if (logits) memcpy(logits + (int64_t)first * V, full.data(), full.size() * 4);
         }
     } catch (...) {
+        cudaStreamSynchronize(d.stream);  // launches that still write to the pages given back here
         K.book.undo_extend(seq, count.data(), n);
         throw;
     }

@@ -164,3 +164,20 @@ def test_refusals_and_cancellation_change_nothing(twin):
     ctx.kv_release(other)
     ctx.kv_release(small)
     ctx.kv_free(kv, [a, b])
+
+
+def test_a_forward_whose_wait_gave_up_changes_nothing(twin):
+    ctx, kv, spec = twin.ctx, twin.kv, twin.spec
+    seqs = ctx.kv_open(kv, 2)
+    first = [ids(spec, 40, 1), ids(spec, 3, 2)]
+    ctx.kv_forward(kv, seqs, first, want_logits=False)
+    used = ctx.kv_info(kv)["pages_used"]
+    chunks = [ids(spec, 20, 3), ids(spec, 1, 4)]
+    ctx.debug_kv_error(kv, 0, 3)
+    with pytest.raises(binding.ShieldError) as e:
+        ctx.kv_forward(kv, seqs, chunks)
+    assert e.value.code == binding.ERR_TIMEOUT
+    assert ctx.kv_lengths(kv, seqs).tolist() == [40, 3] and ctx.kv_info(kv)["pages_used"] == used
+    got = ctx.kv_forward(kv, seqs, chunks)
+    np.testing.assert_array_equal(got, twin.step(seqs, chunks))
+    ctx.kv_free(kv, seqs)
