@@ -1549,7 +1549,7 @@ static void kv_forward(shield_ctx *handle, Ctx &C, int64_t kv_id, const int64_t 
                 B.append.push_back(0);
                 B.tokens += count[k++];
             }
-            kv::Batch &step = kv::model_batch(K, c.n_heads, (int32_t)B.tokens, k - first, longest);
+            kv::Batch &step = kv::model_batch(K, c.n_heads, (int32_t)B.tokens, k - first, longest, c.max_batch_tokens, c.max_positions);
             kv::set_batch(step, seq + first, count.data() + first, k - first, d.stream);
             packed.assign(ids + offsets[first], ids + offsets[k]);
             full.resize((size_t)(k - first) * V);

@@ -217,18 +217,21 @@ static void batch_create(shield_ctx *ctx, int64_t kv, const shield_kv_batch_conf
     st.batches.emplace(*out, std::move(B));
 }
 
-Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions) {
+Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions, int32_t most_tokens, int32_t most_positions) {
     Batch *b = c.model.get();
     if (b && b->n_heads == n_heads && b->max_tokens >= tokens && b->max_seqs >= seqs && b->max_positions >= positions) return *b;
-    shield_kv_batch_config cfg{n_heads, tokens, seqs, positions};
-    if (b && b->n_heads == n_heads) {
-        cfg.max_tokens = std::max(cfg.max_tokens, b->max_tokens);
-        cfg.max_seqs = std::max(cfg.max_seqs, b->max_seqs);
-        cfg.max_positions = std::max(cfg.max_positions, b->max_positions);
-    }
+    const bool grows = b && b->n_heads == n_heads;
+    // (a step has no more sequences than tokens)
+    const shield_kv_batch_config need{n_heads, tokens, seqs, positions},
+        roomy{n_heads, grown(grows ? b->max_tokens : 0, tokens, most_tokens), grown(grows ? b->max_seqs : 0, seqs, most_tokens),
+              grown(grows ? b->max_positions : 0, positions, most_positions)};
     SHIELD_CUDA(cudaStreamSynchronize(c.dev.stream));
     c.model.reset();
-    c.model = make_batch(c, &cfg);
+    try {
+        c.model = make_batch(c, &roomy);
+    } catch (const Error &) {  // no memory for that much
+        c.model = make_batch(c, &need);
+    }
     return *c.model;
 }
 

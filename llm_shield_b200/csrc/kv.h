@@ -46,8 +46,9 @@ struct Batch {
 };
 
 // The cache's batch for the model's own forwards, with room for a step of this
-// size (made anew, once the GPU is done with it, when it has to grow).
-Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions);
+// size: made anew, once the GPU is done with it, when it has to grow, and then
+// with room for more, up to steps of most_tokens and sequences of most_positions.
+Batch &model_batch(Cache &c, int32_t n_heads, int32_t tokens, int32_t seqs, int32_t positions, int32_t most_tokens, int32_t most_positions);
 // Plans a step on the context's stream; the calls below are one layer of it.
 void set_batch(Batch &B, const int64_t *seqs, const int32_t *counts, int32_t n, cudaStream_t s);
 void write_layer(Batch &B, int32_t layer, const float *k, const float *v, cudaStream_t s);

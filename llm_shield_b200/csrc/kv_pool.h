@@ -278,6 +278,16 @@ private:
     std::vector<int32_t> idle_;    // slots without a sequence
 };
 
+// The capacity to make for `need` where there is room for `have`: a power of
+// two up to `most`, so that a sequence that grows by a token a step outgrows it
+// a few times in all.
+inline int32_t grown(int32_t have, int32_t need, int32_t most) {
+    if (need <= have) return have;
+    int64_t c = 1;
+    while (c < need) c *= 2;
+    return (int32_t)std::max<int64_t>(need, std::min<int64_t>(c, most));
+}
+
 // ------------------------------------------------------------- attention plan
 
 // One piece of attention work for every kv head: rows [r0, r0 + nr) of a

@@ -181,3 +181,18 @@ def test_a_forward_whose_wait_gave_up_changes_nothing(twin):
     got = ctx.kv_forward(kv, seqs, chunks)
     np.testing.assert_array_equal(got, twin.step(seqs, chunks))
     ctx.kv_free(kv, seqs)
+
+
+def test_decode_steps_keep_their_batch(twin):
+    """A word set in the batch of one step is there in the next: the batch has not been made anew for one more position."""
+    ctx, spec = twin.ctx, twin.spec
+    kv = ctx.kv_create(twin.type, spec.n_layers, spec.n_kv_heads, spec.head_dim, 16, 20)
+    seqs = ctx.kv_open(kv, 3)
+    ctx.kv_forward(kv, seqs, [ids(spec, 40, i) for i in range(3)], want_logits=False)
+    for n in range(4):
+        ctx.kv_forward(kv, seqs, [ids(spec, 1, 9 + i) for i in range(3)], want_logits=False)
+        ctx.debug_kv_error(kv, 0, 3)
+        with pytest.raises(binding.ShieldError) as e:
+            ctx.kv_forward(kv, seqs, [ids(spec, 1, 9 + i) for i in range(3)], want_logits=False)
+        assert e.value.code == binding.ERR_TIMEOUT
+    ctx.kv_release(kv)

@@ -412,3 +412,18 @@ def test_a_planned_compaction_changes_nothing_until_it_is_taken(host, pt):
     planned = p.moves()
     np.testing.assert_array_equal(p.compact(), planned)
     assert len(planned) and host.host_spanned(p.h) == host.host_used(p.h) == len(held)
+
+
+def test_capacities_grow_a_few_times(host):
+    rng = random.Random(0)
+    for most in (1, 7, 512, 8192, 2 ** 31 - 1):
+        have = times = 0
+        for need in range(1, min(most, 20000) + 1):
+            now = host.host_grown(have, need, most)
+            assert need <= now <= max(most, need) and now >= have
+            times += now != have
+            have = now
+        assert times <= 16
+        for _ in range(200):
+            have, need = rng.randint(0, most), rng.randint(1, most)
+            assert max(have, need) <= host.host_grown(have, need, most) <= most
