@@ -319,7 +319,9 @@ shield_status shield_kv_batch_set(shield_ctx *ctx, int64_t batch, const int64_t 
  * The step's keys and values of one layer into the pool. k, v: device rows of
  * n_kv_heads * head_dim values, one per token, k_stride / v_stride elements
  * apart (0: packed; 16-byte aligned), SHIELD_TYPE_F32 (rounded to nearest) or
- * the cache's own type.
+ * the cache's own type. A step that reaches back into pages that others share
+ * is written for them as well; SHIELD_ERR_STATE when two of the step's own
+ * sequences share one of its positions.
  */
 shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uint32_t type, const void *k,
                               int64_t k_stride, const void *v, int64_t v_stride, void *stream);

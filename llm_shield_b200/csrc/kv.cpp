@@ -296,6 +296,7 @@ void set_batch(Batch &B, const int64_t *seqs, const int32_t *counts, int32_t n, 
     B.seqs.assign(seqs, seqs + n);
     B.frees = c.book.frees();
     B.moves = c.book.moves();
+    B.meets = steps_meet(c.book, seqs, counts, n);
     B.planned = true;
 }
 
@@ -339,6 +340,7 @@ static void write_rows(Batch &B, int32_t layer, uint32_t type, const void *k, in
     Cache &c = *B.cache;
     check_plan(B);
     check_layer(c, layer);
+    if (B.meets) throw Error(SHIELD_ERR_STATE, "two sequences of the batch share a position of the step: their rows would be written to one place");
     if (type != SHIELD_TYPE_F32 && type != (c.pool.bf16 ? SHIELD_TYPE_BF16 : SHIELD_TYPE_F16))
         throw Error(SHIELD_ERR_UNSUPPORTED, "rows are F32 or of the cache's own type");
     const int64_t width = (int64_t)c.pool.kv_heads * c.pool.dim;

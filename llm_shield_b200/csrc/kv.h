@@ -42,6 +42,7 @@ struct Batch {
     std::vector<int64_t> seqs;    // the sequences it covers
     int64_t frees = 0, moves = 0; // the pool's counts when it was planned
     bool planned = false;
+    bool meets = false;           // two sequences hold a position of the step in common
     ~Batch();
 };
 

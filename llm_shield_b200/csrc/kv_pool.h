@@ -15,6 +15,7 @@
 #include <numeric>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "error.h"
@@ -59,6 +60,7 @@ public:
 
     const Sequence &get(int64_t id) const { return slot(id).s; }
     bool has(int64_t id) const { return find(id) != nullptr; }
+    int32_t holders(int32_t page) const { return ref_[page]; }
 
     void open(int32_t n, int64_t *out) {
         room(n);
@@ -277,6 +279,19 @@ private:
     std::deque<Slot> slots_;
     std::vector<int32_t> idle_;    // slots without a sequence
 };
+
+// Whether two sequences have a page in common among those of their last count[i]
+// positions. (It is full, and the last positions of each reach its end.)
+inline bool steps_meet(const Pool &pool, const int64_t *ids, const int32_t *count, int32_t n) {
+    std::unordered_set<int32_t> seen;
+    for (int32_t i = 0; i < n; i++) {
+        const Sequence &s = pool.get(ids[i]);
+        if (count[i] <= 0) continue;
+        for (size_t j = (size_t)((s.len - count[i]) / pool.page_tokens()); j < s.pages.size(); j++)
+            if (pool.holders(s.pages[j]) > 1 && !seen.insert(s.pages[j]).second) return true;
+    }
+    return false;
+}
 
 // The capacity to make for `need` where there is room for `have`: a power of
 // two up to `most`, so that a sequence that grows by a token a step outgrows it

@@ -90,6 +90,7 @@ int64_t host_plan_array(Host *h, int32_t which, int32_t *out) {
     return -1;
 }
 int32_t host_grown(int32_t have, int32_t need, int32_t most) { return grown(have, need, most); }
+int32_t host_steps_meet(Host *h, const int64_t *ids, const int32_t *c, int32_t n) { return steps_meet(h->pool, ids, c, n); }
 int64_t host_part_rows(Host *h) { return h->plan.part_rows; }
 
 }  // extern "C"

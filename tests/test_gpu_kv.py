@@ -777,3 +777,31 @@ def test_a_wait_that_gave_up_is_told():
         with pytest.raises(binding.ShieldError) as e:
             bad()
         assert e.value.code == binding.ERR_ARG
+
+
+def test_rows_of_two_sequences_are_not_written_to_one_place():
+    c = Cache("f16", 1, 2, 64, 16, pages=40)
+    (root,) = c.ctx.kv_open(c.kv, 1)
+    c.ctx.kv_extend(c.kv, [root], [32])
+    kids = c.ctx.kv_fork(c.kv, [root] * 2, stream=c.stream)
+    c.ctx.kv_extend(c.kv, kids, [3, 5])
+    before = c.k.clone()
+    k = torch.randn(48, 2, 64, device="cuda")
+    b = c.batch(kids, [3, 5], 4, max_tokens=48)
+
+    def write():
+        c.ctx.kv_write(b, 0, k.data_ptr(), k.data_ptr(), "f32", stream=c.stream)
+
+    for counts in ([4, 6], [35, 6], [3, 37]):  # back into the shared pages: both, both, one of them
+        c.ctx.kv_batch_set(b, kids, counts, stream=c.stream)
+        if counts[0] == 3:
+            write()
+            assert torch.equal(c.rows(root, 0, c.k), k[3:35].half())
+            continue
+        with pytest.raises(binding.ShieldError) as e:
+            write()
+        assert e.value.code == binding.ERR_STATE
+        assert torch.equal(c.k, before)
+    c.ctx.kv_batch_set(b, kids, [3, 5], stream=c.stream)
+    write()
+    check(c, kids, [4, 6], 4, layer=0)  # queries of shared positions are no conflict

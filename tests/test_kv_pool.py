@@ -427,3 +427,24 @@ def test_capacities_grow_a_few_times(host):
         for _ in range(200):
             have, need = rng.randint(0, most), rng.randint(1, most)
             assert max(have, need) <= host.host_grown(have, need, most) <= most
+
+
+def test_steps_that_meet_on_a_page(host):
+    """Against the slots of the plan: a meeting is a slot that appears twice."""
+    host.host_steps_meet.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32]
+    rng, seen = random.Random(5), set()
+    for _ in range(150):
+        p = HostPool(host, 400, 16)
+        ids = list(p.open(3))
+        p.extend(ids, [rng.randint(0, 70) for _ in ids])
+        for _ in range(2):
+            ids += list(p.fork(rng.choices(ids, k=3)))
+            p.extend(ids, [rng.choice((0, 0, 1, 16, 20)) for _ in ids])
+        batch = rng.sample(ids, rng.randint(1, 6))
+        counts = [min(p.length(i), rng.choice((0, 1, 5, 16, 40))) for i in batch]
+        slots = p.plan(batch, counts)["slot"]
+        twice = len(set(slots.tolist())) < len(slots)
+        i, c = np.asarray(batch, np.int64), np.asarray(counts, np.int32)
+        assert bool(host.host_steps_meet(p.h, i.ctypes.data, c.ctypes.data, len(batch))) == twice
+        seen.add(twice)
+    assert seen == {True, False}
