@@ -46,7 +46,7 @@ public:
     int32_t page_tokens() const { return page_tokens_; }
     int32_t n_pages() const { return (int32_t)ref_.size(); }
     int32_t pages_used() const { return n_pages() - free_count_; }
-    int32_t sequences() const { return (int32_t)(slots_.size() - idle_.size()); }
+    int32_t sequences() const { return (int32_t)(slots_.size() - idle_.size()) - spent_; }
     // One past the highest page in use.
     int32_t pages_spanned() const {
         int32_t p = n_pages();
@@ -146,8 +146,8 @@ public:
             t.s.pages.clear();  // keeps its memory for the slot's next sequence
             t.s.len = 0;
             t.live = false;
-            t.turn = (t.turn + 1) & TURN_MASK;
-            idle_.push_back((int32_t)(ids[i] & SLOT_MASK));
+            if (++t.turn <= TURN_MASK) idle_.push_back((int32_t)(ids[i] & SLOT_MASK));
+            else spent_++;  // its ids are used up: one that ended long ago must not name another sequence
         }
         if (n > 0) frees_++;
     }
@@ -278,6 +278,7 @@ private:
     size_t hint_ = 0;              // no free page in a word before this one
     std::deque<Slot> slots_;
     std::vector<int32_t> idle_;    // slots without a sequence
+    int32_t spent_ = 0;            // slots that take no sequence any more
 };
 
 // Whether two sequences have a page in common among those of their last count[i]

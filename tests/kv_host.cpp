@@ -91,6 +91,19 @@ int64_t host_plan_array(Host *h, int32_t which, int32_t *out) {
 }
 int32_t host_grown(int32_t have, int32_t need, int32_t most) { return grown(have, need, most); }
 int32_t host_steps_meet(Host *h, const int64_t *ids, const int32_t *c, int32_t n) { return steps_meet(h->pool, ids, c, n); }
+// n sequences opened and freed one after another: how many had the id of the first or of the one before
+int64_t host_churn(Host *h, int64_t n) {
+    int64_t first = 0, last = 0, id = 0, again = 0;
+    for (int64_t i = 0; i < n; i++) {
+        h->pool.open(1, &id);
+        if (i == 0) first = id;
+        else again += id == first || id == last;
+        last = id;
+        h->pool.free(&id, 1);
+    }
+    return again;
+}
+int32_t host_sequences(Host *h) { return h->pool.sequences(); }
 int64_t host_part_rows(Host *h) { return h->plan.part_rows; }
 
 }  // extern "C"

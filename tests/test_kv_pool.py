@@ -448,3 +448,20 @@ def test_steps_that_meet_on_a_page(host):
         assert bool(host.host_steps_meet(p.h, i.ctypes.data, c.ctypes.data, len(batch))) == twice
         seen.add(twice)
     assert seen == {True, False}
+
+
+def test_an_id_is_never_given_twice(host):
+    """Past the turns that an id counts, a slot is left alone and the next one is taken."""
+    host.host_churn.argtypes, host.host_churn.restype = [C.c_void_p, C.c_int64], C.c_int64
+    p = HostPool(host, 8, 16)
+    (first,) = p.open(1)
+    p.free([first])
+    assert host.host_churn(p.h, (1 << 22) + 5) == 0  # pairs of open and free that gave an id of an earlier one again
+    (now,) = p.open(1)
+    assert now != first
+    with pytest.raises(binding.ShieldError):
+        p.extend([first], [1])
+    p.extend([now], [3])
+    assert host.host_used(p.h) == 1 and host.host_sequences(p.h) == 1
+    p.free([now])
+    assert host.host_used(p.h) == 0 and host.host_sequences(p.h) == 0
