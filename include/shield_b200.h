@@ -331,12 +331,13 @@ shield_status shield_kv_write(shield_ctx *ctx, int64_t batch, int32_t layer, uin
  * over the positions l of its sequence up to and including its own. q, out:
  * device rows of n_heads * head_dim values of the cache's type, q_stride /
  * out_stride elements apart (0: packed; 16-byte aligned); query head h reads
- * kv head h / (n_heads / n_kv_heads). out may be q. Keys and values behind a
- * token's position have no effect on it, whatever they hold. Scores and sums
- * are f32, weights are rounded to the cache's type for the product with the
- * values. The order of the sums, and so the last bits, depend on how the plan
- * cuts the work: on the batch's lengths and on what is shared; the same plan
- * gives the same bits.
+ * kv head h / (n_heads / n_kv_heads). out may be q, with q's
+ * stride, and overlaps it in no other way (SHIELD_ERR_ARG). Keys and values
+ * behind a token's position have no effect on it, whatever they hold. Scores
+ * and sums are f32, weights are rounded to the cache's type for the product
+ * with the values. The order of the sums, and so the last bits, depend on how
+ * the plan cuts the work: on the batch's lengths, on what is shared and on the
+ * batch's capacities; the same plan gives the same bits.
  */
 shield_status shield_kv_attend(shield_ctx *ctx, int64_t batch, int32_t layer, const void *q, int64_t q_stride, void *out,
                                int64_t out_stride, float scale, void *stream);

@@ -335,6 +335,19 @@ static int64_t row_stride(int64_t stride, int64_t width, const void *p, int elt,
     return stride;
 }
 
+// Whether some of `tokens` output rows may lie over the queries of another token
+// or head: not where the two are one array, lie apart, or take turns in rows of
+// one stride.
+static bool rows_clash(const void *q, int64_t q_stride, const void *out, int64_t out_stride, int64_t width, int64_t tokens) {
+    if (tokens == 0 || (q == out && (tokens == 1 || q_stride == out_stride))) return false;
+    const int64_t a = (int64_t)reinterpret_cast<uintptr_t>(q), b = (int64_t)reinterpret_cast<uintptr_t>(out);
+    const int64_t a_end = a + ((tokens - 1) * q_stride + width) * 2, b_end = b + ((tokens - 1) * out_stride + width) * 2;
+    if (a_end <= b || b_end <= a) return false;
+    if (q_stride != out_stride) return true;
+    const int64_t row = q_stride * 2, off = ((b - a) % row + row) % row;
+    return off < width * 2 || off > row - width * 2;
+}
+
 static void write_rows(Batch &B, int32_t layer, uint32_t type, const void *k, int64_t k_stride, const void *v,
                        int64_t v_stride, cudaStream_t s) {
     Cache &c = *B.cache;
@@ -367,6 +380,10 @@ static void attend(Batch &B, int32_t layer, const void *q, int64_t q_stride, voi
     if (!cap && B.last.perm.empty()) return;
     A.q_stride = row_stride(q_stride, width, q, 2, "q");
     A.out_stride = row_stride(out_stride, width, out, 2, "out");
+    // (captured: later plans' tokens are not known, so only what clashes from two on)
+    if (cap ? q == out && A.q_stride != A.out_stride && B.max_tokens > 1
+            : rows_clash(q, A.q_stride, out, A.out_stride, width, (int64_t)B.last.perm.size()))
+        throw Error(SHIELD_ERR_ARG, "out overlaps q (it may be q, with q's stride)");
     A.pool = c.pool;
     A.plan = B.plan;
     A.q = q;

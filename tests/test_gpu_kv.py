@@ -805,3 +805,37 @@ def test_rows_of_two_sequences_are_not_written_to_one_place():
     c.ctx.kv_batch_set(b, kids, [3, 5], stream=c.stream)
     write()
     check(c, kids, [4, 6], 4, layer=0)  # queries of shared positions are no conflict
+
+
+def test_outputs_over_other_queries_are_refused():
+    c = Cache("bf16", 1, 2, 64, 16, pages=40)
+    (s,) = c.ctx.kv_open(c.kv, 1)
+    c.ctx.kv_extend(c.kv, [s], [60])
+    b = c.batch([s], [40], 4)
+    w = 4 * 64
+    x = torch.randn(200, 2 * w, device="cuda").to(c.dtype)
+    q = x[:40, :w].clone()
+    want, tol = expect(c, [s], [40], q.view(40, 4, 64), 0, 0.125)
+
+    def attend(offset, q_stride, out_stride):
+        x[:40 * q_stride // (2 * w) + 1].view(-1)[:40 * q_stride].view(40, q_stride)[:, :w] = q
+        base = x.data_ptr()
+        c.ctx.kv_attend(b, 0, base, base + 2 * offset, 0.125, q_stride=q_stride, out_stride=out_stride, stream=c.stream)
+        out = torch.as_strided(x, (40, w), (out_stride, 1), offset)
+        assert ((out.double().view(40, 4, 64) - want).abs() <= tol).all()
+
+    attend(0, w, w)
+    attend(0, 2 * w, 2 * w)
+    attend(w, 2 * w, 2 * w)  # rows that take turns
+    attend(40 * w, w, 2 * w)
+    attend(40 * 2 * w, 2 * w, w)
+    for offset, q_stride, out_stride in [(0, w, 2 * w), (0, 2 * w, w), (8, w, w), (w // 2, w, w), (w - 8, 2 * w, 2 * w), (w + 8, 2 * w, 2 * w),
+                                         (39 * w, w, 2 * w), (w, 2 * w, w)]:
+        with pytest.raises(binding.ShieldError) as e:
+            attend(offset, q_stride, out_stride)
+        assert e.value.code == binding.ERR_ARG
+    c.ctx.kv_batch_set(b, [s], [1], stream=c.stream)
+    one = x[0].clone()
+    c.ctx.kv_attend(b, 0, x.data_ptr(), x.data_ptr(), 0.125, q_stride=w, out_stride=2 * w, stream=c.stream)
+    want, tol = expect(c, [s], [1], one[:w].view(1, 4, 64), 0, 0.125)
+    assert ((x[0, :w].double().view(1, 4, 64) - want).abs() <= tol).all()
