@@ -463,10 +463,12 @@ static void ensure_buffers(Ctx &C, Device &d) {
     SHIELD_CUDA(cudaMallocHost((void **)&d.buf.h_meta, (size_t)(4 * T) * 4));
     SHIELD_CUDA(cudaMallocHost((void **)&d.buf.h_logits, (size_t)(T * 64) * 4));
     // attention scratch: at least one work item of the longest request, at
-    // most 4 GiB (a micro-batch needing more is attended in several launches)
+    // most 4 GiB (a micro-batch needing more is attended in several launches); a
+    // paged forward's queries and outputs take the same place
     int64_t one = attention_scratch_floats(c.max_positions, c.n_kv_heads, attention_rows_per_cta());
     int64_t all = std::min<int64_t>((int64_t)1 << 30, (int64_t)c.n_heads * T * c.max_positions);
-    d.buf.scores_cap = std::max(one, all);
+    const int64_t paged = std::min<int64_t>((int64_t)1 << 30, T * c.qdim());
+    d.buf.scores_cap = std::max({one, all, paged});
     dev_alloc(d.buf.scores, (size_t)d.buf.scores_cap);
     dev_alloc(d.buf.att, (size_t)(ATT_INTS_PER_TOKEN * T + ATT_INTS_EXTRA));
     SHIELD_CUDA(cudaMallocHost((void **)&d.buf.h_att, (size_t)(ATT_INTS_PER_TOKEN * T + ATT_INTS_EXTRA) * 4));

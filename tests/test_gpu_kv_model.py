@@ -196,3 +196,16 @@ def test_decode_steps_keep_their_batch(twin):
             ctx.kv_forward(kv, seqs, [ids(spec, 1, 9 + i) for i in range(3)], want_logits=False)
         assert e.value.code == binding.ERR_TIMEOUT
     ctx.kv_release(kv)
+
+
+def test_a_model_of_few_positions(twin):
+    """Paged forwards where the exact attention's scratch for so few positions would not hold a batch's queries and outputs."""
+    ctx = binding.ShieldContext(1)
+    ctx.set_config(twin.spec, max_positions=64, max_batch_tokens=600)
+    ctx.upload_model(twin.t)
+    small = Twin(ctx, twin.spec, twin.t, twin.type)
+    seqs = ctx.kv_open(small.kv, 12)
+    for chunks in ([ids(twin.spec, 50 - i, i) for i in range(12)], [ids(twin.spec, 14, 20 + i) for i in range(12)]):
+        got = ctx.kv_forward(small.kv, seqs, chunks)
+        np.testing.assert_array_equal(got, small.step(seqs, chunks))
+    ctx.close()
