@@ -229,7 +229,9 @@ shield_status shield_seq_release(shield_ctx *ctx, int64_t seq);
  * Streams: `stream` is the cudaStream_t on which a call enqueues its GPU work,
  * null for the context's own stream of that GPU (cudaStreamLegacy names the
  * default stream). No call here waits for the GPU, except that creating and
- * releasing may. Bookkeeping happens at the call, so calls on one cache that
+ * releasing may, shield_kv_batch_set waits until the upload of the last plan
+ * but one has left its staging memory, and shield_kv_forward waits for its
+ * results. Bookkeeping happens at the call, so calls on one cache that
  * use different streams are ordered by the caller (events), a page freed in
  * one call and handed out in the next among them. Device pointers belong to
  * the cache's GPU, whichever device is current; the current device is left as
@@ -354,12 +356,12 @@ shield_status shield_kv_batch_check(shield_ctx *ctx, int64_t batch);
  * max_batch_tokens on the context's stream of the cache's GPU, and writes each
  * sequence's whole tied head at its new last position to logits[i * vocab ..]
  * when logits is non-null. Keys and values are the exact path's, rounded to
- * the cache's type; the attention is shield_kv_attend's, on queries rounded
- * to that type, so logits differ from the exact path's in their last digits
- * and follow the batch's plan. Everything else is bit-identical to it. If the
- * call fails, no sequence has changed. SHIELD_ERR_RANGE beyond max_positions,
- * SHIELD_ERR_NOMEM when the pool has too few pages. The cache's contents are
- * its user's: they are kept when weights are uploaded again.
+ * the cache's type; the attention is shield_kv_attend's, whose queries and
+ * outputs are of that type, so logits differ from the exact path's in their
+ * last digits and follow the batch's plan. Everything else is bit-identical to
+ * it. If the call fails, no sequence has changed. SHIELD_ERR_RANGE beyond
+ * max_positions, SHIELD_ERR_NOMEM when the pool has too few pages. The cache's
+ * contents are its user's: they are kept when weights are uploaded again.
  */
 shield_status shield_kv_forward(shield_ctx *ctx, int64_t kv, const int64_t *seqs, const int32_t *ids,
                                 const int64_t *offsets, int32_t n, float *logits, const volatile int32_t *cancel);

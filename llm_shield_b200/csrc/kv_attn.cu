@@ -344,10 +344,11 @@ cudaError_t launch_attend_few(const AttendArgs &A, int64_t units, bool beside, c
 // ----------------------------------------------------------------- joining
 
 // One warp per (token, query head): 11 partials of 4096 rows of 128 in 6.7 us.
-// The row's partials lie one per piece of
-// keys of each segment on the way from the sequence's own keys up through the
-// runs it shares, always in that order. A lane looks up one piece, so that the
-// lookups of up to 32 pieces and the reads of their outputs go out together.
+// The row's partials lie one per piece of keys of each segment on the way from
+// the sequence's own keys up through the runs it shares, always in that order.
+// A lane looks up one piece, so that the lookups of up to 32 pieces and the
+// reads of their outputs go out together. (Dim 64: 32 registers, 12 bytes
+// spilled.)
 template <bool BF16, int D>
 __global__ void __launch_bounds__(128) k_attend_merge(const AttendArgs A) {
     using H = Half16<BF16>;

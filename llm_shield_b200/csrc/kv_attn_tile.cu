@@ -7,14 +7,13 @@
 //   S = Q K^T   tcgen05.mma, both operands in shared memory, S in TMEM
 //   P = 2^(scale S - m), rounded to the cache's type, over S's own TMEM columns
 //   O += P V    tcgen05.mma with P read from TMEM, O (f32) in TMEM
-// The exponential unit is as scarce as the tensor pipe (16 per SM and cycle:
-// 1024 cycles for the 128 x 128 weights that two products of 512 cycles each
-// use), so a quarter of the exponentials go to the FMA pipe, and a tile's
-// scores come in halves of 64 keys: one half's are there while the other's are
-// turned into weights, which TMEM has no room for at 128 (S, S, O, O fill its
-// 512 columns). Up to 128 rows there is one row tile and
-// the two take alternate key blocks, each with its own (m, sum, O), joined at
-// the end.
+// A tile's scores come in halves of 64 keys: one half's are there while the
+// other's are turned into weights, which TMEM has no room for at 128 (S, S, O, O
+// fill its 512 columns). The exponential unit needs as many cycles as the two
+// products (1024 for 128 x 128 weights at 16 a cycle); a quarter of the
+// exponentials go to the FMA pipe instead. Up to 128 rows there is one row tile
+// and the two warpgroups take alternate key blocks, each with its own (m, sum,
+// O), joined at the end.
 //
 //   warps 0-3, 4-7  one softmax warpgroup per tile, a thread per row: turns S
 //                   into P, rescales O when the row's maximum has grown by more
@@ -29,9 +28,11 @@
 // what it needs is there.
 //
 // Measured: 3 prompts of 4096 tokens, 32 query and 8 kv heads of 128, bf16, in
-// 435 us (950 TFLOP/s of causal pairs) at the power cap, 375-400 us cool. No
+// 433 us (950 TFLOP/s of causal pairs) at the power cap, 375-400 us cool. No
 // unit is saturated (tensor pipe 56%, exponentials 42%, issue 44%): each
-// softmax warp waits on its own chain, and the clock falls to 1650 MHz.
+// softmax warp waits on its own chain (load, maximum, exponentials, store,
+// hand-over), and the clock falls to 1650 MHz. At dim 64 the compiler
+// spills 48 bytes a thread.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -56,8 +57,10 @@ constexpr int TILE_THREADS = 384;
 constexpr int ROWS = 128;      // rows of a tile
 constexpr int BLOCK = 128;     // keys of a block, the step of the ring
 constexpr int HALF = 64;       // keys of one score product: a tile's S has room for two
-// One in this many pairs of weights is computed on the FMA pipe (3 prompts of
-// 4096: none 445 us, every 8th 445, 4th 442, 3rd 439; every 2nd was slower by 5%).
+// One in this many pairs of weights is computed on the FMA pipe. It matters
+// little while neither unit bounds the kernel (3 prompts of 4096: none 445 us,
+// every 8th 445, 4th 442, 3rd 439, within a few us of one another from run to
+// run); every 2nd was slower by 5%.
 constexpr int POLY_EVERY = 4;
 constexpr float GROWTH = 8.0f; // log2 of how far a maximum may grow before O is rescaled
 

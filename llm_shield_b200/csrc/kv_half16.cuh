@@ -17,8 +17,11 @@ template <bool BF16>
 struct Half16;
 template <>
 struct Half16<false> {
-    // f16 weights carry a factor 2^14 (it cancels in o / sum): a weight of 2^-38
-    // of the row's largest is still a number, and the largest is far from overflow
+    // f16 weights carry a factor (it cancels in o / sum), so that small ones are
+    // still numbers and the largest is far from overflow: 2^14 in the few-row
+    // kernel, where the row's largest weight is 1 (down to 2^-38 of it), 2^6 in the
+    // many-row kernel, where the largest may have grown to 2^8 (down to 2^-30 of a
+    // maximum just taken; below 2^-20 of it with fewer bits)
     static constexpr float LIFT = 14.0f;
     static constexpr uint32_t EXP = 0x7C00u;  // exponent bits: all ones in infinities and NaN
     static __device__ __forceinline__ uint32_t pack(float a, float b) {

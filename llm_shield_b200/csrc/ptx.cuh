@@ -35,8 +35,6 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     return ok != 0;
 }
 
-// Bounded wait: gives up after ~2 s of SM clock, raising the CTA's abort flag
-// and the kernel's error word, so a lost arrival can never hang the GPU.
 // Non-blocking test of a phase (the first look of a bounded wait, which on
 // the hot path usually finds the phase complete).
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
@@ -50,6 +48,8 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Bounded wait: gives up after ~2 s of SM clock, raising the CTA's abort flag
+// and the kernel's error word, so a lost arrival can never hang the GPU.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag, int32_t *err) {
     if (mbar_test(bar, parity)) return true;
     long long t0 = clock64();
