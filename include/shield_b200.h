@@ -313,7 +313,8 @@ shield_status shield_kv_batch_release(shield_ctx *ctx, int64_t batch);
  * (SHIELD_ERR_STATE from then on). It cannot be captured into a graph, but
  * shield_kv_write and shield_kv_attend can: a replay works on the plan set
  * last before it, of any size within the capacities, and the caller sees to it
- * that this plan still holds and that the buffers captured are large enough.
+ * that this plan still holds, that a captured write may be made on it and that
+ * the buffers captured are large enough.
  */
 shield_status shield_kv_batch_set(shield_ctx *ctx, int64_t batch, const int64_t *seqs, const int32_t *counts, int32_t n,
                                   void *stream);
